@@ -1,4 +1,5 @@
-"""ctypes binding of build/libgpu_kernels_nvfp4_bench.so (declarations: include/nvfp4_capi.h).
+"""ctypes binding of build/libgpu_kernels_nvfp4_bench.so (declarations: include/nvfp4_capi.h,
+include/operators_capi.h).
 
 The library is the product; there is no Python or CPU fallback. Importing this
 module without the built library raises, and every compute call raises on a
@@ -77,6 +78,22 @@ SIGNATURES = {
     "gpu_kernels_nvfp4_launch_count": ([], ctypes.c_ulonglong),
 }
 
+L = ctypes.c_longlong
+# the int8 and token-routing operators; mirrors include/operators_capi.h one to one
+OPERATOR_SIGNATURES = {
+    "gpu_kernels_int8_quantize": ([P, I, P, P, L, I, P], I),
+    "gpu_kernels_int8_dequantize": ([P, P, P, L, I, P], I),
+    "gpu_kernels_int8_gemm": ([P, P, P, P, P, I, I, I, I, P], I),
+    "gpu_kernels_int8_linear": ([P, I, P, P, P, P, P, I, I, I, I, P], I),
+    "gpu_kernels_int8_grouped_gemm": ([P, P, P, P, P, I, P, I, I, I, I, I, P], I),
+    "gpu_kernels_int8_tiles": ([I, I, I, I, ctypes.POINTER(I)], I),
+    "gpu_kernels_tokens_sort": ([P, I, I, I, P, P, P, P], I),
+    "gpu_kernels_tokens_gather": ([P, I, I, I, I, P, P, P, P], I),
+    "gpu_kernels_tokens_gather_int8": ([P, I, I, I, I, P, P, P, P, P], I),
+    "gpu_kernels_tokens_combine": ([P, I, P, P, P, I, I, I, P, P], I),
+    "gpu_kernels_tokens_combine_backward": ([P, I, P, P, P, P, I, I, I, P, P, P], I),
+}
+
 _lib = None
 
 
@@ -92,7 +109,7 @@ def load() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m gpu_kernels_b200.build` "
                 "(there is no fallback path)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (argtypes, restype) in SIGNATURES.items():
+        for name, (argtypes, restype) in {**SIGNATURES, **OPERATOR_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = argtypes, restype
         _lib = lib

@@ -1,0 +1,317 @@
+// Per-token int8 quantiser, the same into expert order, and the dequantiser, for sm_100a.
+//
+// Row r of x [rows, K]: amax = max |x|, scale = amax / 127 (FP32), code = the integer nearest to 127 x / amax, ties to
+// the even one. The quotient is the exact one, so that a value on a border gets the code the definition gives it (with
+// amax = 2x, for example, 127 x / amax is 63.5): see code_of. A zero row has scale 0 and codes 0. A row that holds a NaN
+// or an infinity has scale NaN and codes 0: what is computed from it is NaN, not a number that looks sound.
+//
+// HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes. Threads take 16
+// values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
+// and stores are aligned whatever K is; a row that starts or ends inside a group takes that group value by value.
+#include "operators_internal.h"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+namespace nvfp4_b200 {
+namespace {
+
+template <typename T> struct Bits;                              // magnitude of a value as an ordered unsigned integer
+template <> struct Bits<__nv_bfloat16> {
+    static constexpr uint32_t NOT_FINITE = 0x7F80u;
+    static __device__ float widen(uint32_t b) { return __uint_as_float(b << 16); }
+};
+template <> struct Bits<__half> {
+    static constexpr uint32_t NOT_FINITE = 0x7C00u;
+    static __device__ float widen(uint32_t b) { return __half2float(__ushort_as_half(static_cast<unsigned short>(b))); }
+};
+template <> struct Bits<float> {
+    static constexpr uint32_t NOT_FINITE = 0x7F800000u;
+    static __device__ float widen(uint32_t b) { return __uint_as_float(b); }
+};
+
+// What a row's codes are made with. f = a power of two that keeps products and quotients of rows of very large or very
+// small values inside FP32's normal range; 1 for all others.
+struct RowScale {
+    float amax, times, divisor, reciprocal;                     // times = 127 f, divisor = amax f, reciprocal = 1 / divisor
+    __device__ RowScale(float a) : amax(a) {
+        const float f = a > 0x1p100f ? 0x1p-64f : a < 0x1p-60f ? 0x1p64f : 1.0f;
+        times = 127.0f * f;
+        divisor = a * f;
+        reciprocal = a > 0.0f ? 1.0f / divisor : 0.0f;
+    }
+};
+
+constexpr float ROUND = 12582912.0f;                            // 1.5 * 2^23: adding it rounds to an integer, ties to even, in the low bits
+
+// 127 x / amax rounded to an integer, in the low byte of the result. 16-bit inputs: p = 127 x is exact (at most 18
+// significant bits). q0 = p * reciprocal is within 2 ulp of the quotient; its residual p - q0 * amax is exact in an FMA,
+// and one correction gives the quotient rounded once: exactly k + 1/2 where that is the quotient, and never k + 1/2
+// elsewhere, since a quotient of such operands that is no tie lies at least 2^-19 (relative) away from one. FP32 inputs:
+// p is rounded, so a quotient within 2^-14 of a tie is decided by comparing 127 |x| with (k + 1/2) amax, both exact in
+// 64 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
+    const float p = x * s.times;
+    const float q0 = p * s.reciprocal;
+    float q = __fmaf_rn(__fmaf_rn(-q0, s.divisor, p), s.reciprocal, q0);
+    if constexpr (sizeof(T) == 4) {
+        const float n = rintf(q);
+        if (fabsf(q - n) > 0.5f - 0x1p-14f) {
+            const float k = floorf(fabsf(q));
+            const double value = 127.0 * fabs(double(x)), tie = (double(k) + 0.5) * double(s.amax);
+            const float low_even = k - 2.0f * floorf(0.5f * k);
+            q = copysignf(value > tie || (value == tie && low_even != 0.0f) ? k + 1.0f : k, q);
+        }
+    }
+    return __float_as_uint(q + ROUND);
+}
+
+template <typename T>
+struct Group {                                                  // 16 values as loaded
+    uint4 raw[sizeof(T)];
+
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4& v = raw[i / 4];
+        return i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w;
+    }
+    __device__ __forceinline__ void load(const T* x, size_t group) {
+        const uint4* p = reinterpret_cast<const uint4*>(x + group * 16);
+        #pragma unroll
+        for (int i = 0; i < int(sizeof(T)); ++i) raw[i] = __ldg(p + i);
+    }
+    // Only the elements [begin, end) of the flat array; zeros for the others, which raise no maximum.
+    __device__ __forceinline__ void load_part(const T* x, size_t group, size_t begin, size_t end) {
+        using U = typename std::conditional<sizeof(T) == 2, unsigned short, uint32_t>::type;
+        const U* p = reinterpret_cast<const U*>(x);
+        uint32_t w[4 * sizeof(T)];
+        #pragma unroll
+        for (int i = 0; i < int(4 * sizeof(T)); ++i) w[i] = 0u;
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const size_t at = group * 16 + i;
+            const uint32_t v = at >= begin && at < end ? uint32_t(__ldg(p + at)) : 0u;
+            if constexpr (sizeof(T) == 2) w[i / 2] |= v << (16 * (i % 2));
+            else w[i] = v;
+        }
+        #pragma unroll
+        for (int i = 0; i < int(sizeof(T)); ++i) raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+    __device__ __forceinline__ uint32_t magnitude(uint32_t sofar) const {   // 16-bit types: two maxima side by side
+        #pragma unroll
+        for (int i = 0; i < int(4 * sizeof(T)); ++i) {
+            if constexpr (sizeof(T) == 2) sofar = __vmaxu2(sofar, word(i) & 0x7FFF7FFFu);
+            else sofar = max(sofar, word(i) & 0x7FFFFFFFu);
+        }
+        return sofar;
+    }
+    __device__ __forceinline__ uint4 codes(const RowScale& s) const {
+        uint32_t out[4];
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t c[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = 4 * q + i;
+                float x;
+                if constexpr (sizeof(T) == 2) x = Bits<T>::widen(at % 2 ? word(at / 2) >> 16 : word(at / 2) & 0xFFFFu);
+                else x = Bits<T>::widen(word(at));
+                c[i] = code_of<T>(x, s);
+            }
+            out[q] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        }
+        return make_uint4(out[0], out[1], out[2], out[3]);
+    }
+};
+
+// TPR: threads per row, NV: groups of 16 that each of them holds in registers (0: any number, the row is read twice, the
+// second time from L2). ROUTED: the row's codes go to `topk` rows of the output instead of its own.
+template <typename T, int TPR, int NV, bool ROUTED>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, long long rows, int K,
+                     const int* __restrict__ position, const int* __restrict__ live, int topk) {
+    ptx::chain_point();
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, ROWS = THREADS / TPR;
+    const int t = threadIdx.x % TPR;
+    const long long row = (long long)(blockIdx.x) * ROWS + threadIdx.x / TPR;
+    if (TPR == 32 && row >= rows) return;                       // (a warp's row; otherwise the grid has one block per row)
+    const size_t begin = size_t(row) * K, end = begin + K;
+    const size_t g0 = begin / 16, g1 = (end + 15) / 16;
+    auto fetch = [&](Group<T>& v, size_t group) {
+        if (group * 16 >= begin && group * 16 + 16 <= end) v.load(x, group);
+        else v.load_part(x, group, begin, end);
+    };
+    Group<T> held[NV > 0 ? NV : 1];
+    uint32_t top = 0u;
+    if constexpr (NV > 0) {
+        #pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (g0 + t + j * TPR < g1) fetch(held[j], g0 + t + j * TPR);
+        #pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (g0 + t + j * TPR < g1) top = held[j].magnitude(top);
+    } else {
+        for (size_t group = g0 + t; group < g1; group += TPR) {
+            fetch(held[0], group);
+            top = held[0].magnitude(top);
+        }
+    }
+    if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if constexpr (TPR > 32) {
+        __shared__ uint32_t warp_top[TPR / 32];
+        if (threadIdx.x % 32 == 0) warp_top[threadIdx.x / 32] = top;
+        __syncthreads();
+        const uint32_t mine = threadIdx.x % 32 < TPR / 32 ? warp_top[threadIdx.x % 32] : 0u;
+        top = __reduce_max_sync(0xFFFFFFFFu, mine);
+    }
+    const bool finite = top < Bits<T>::NOT_FINITE;
+    const RowScale s(finite ? Bits<T>::widen(top) : 0.0f);
+    const float scale = finite ? s.amax / 127.0f : __int_as_float(0x7FC00000);
+    auto emit = [&](const Group<T>& v, size_t group) {
+        const uint4 c = finite ? v.codes(s) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (ROUTED) {                                  // K is a multiple of 16: whole groups
+            const long long out_rows = rows * topk;
+            const int end_live = __ldg(live);
+            for (int j = 0; j < topk; ++j) {
+                const int to = __ldg(position + row * topk + j);
+                if (to < 0 || to >= out_rows) continue;
+                reinterpret_cast<uint4*>(codes)[size_t(to) * (K / 16) + (group - g0)] = to < end_live ? c : make_uint4(0u, 0u, 0u, 0u);
+            }
+        } else if (group * 16 >= begin && group * 16 + 16 <= end) {
+            reinterpret_cast<uint4*>(codes)[group] = c;
+        } else {
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            #pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (group * 16 + i >= begin && group * 16 + i < end) codes[group * 16 + i] = int8_t(w[i / 4] >> (8 * (i % 4)));
+        }
+    };
+    if constexpr (NV > 0) {
+        #pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (g0 + t + j * TPR < g1) emit(held[j], g0 + t + j * TPR);
+    } else {
+        for (size_t group = g0 + t; group < g1; group += TPR) {
+            fetch(held[0], group);
+            emit(held[0], group);
+        }
+    }
+    if constexpr (ROUTED) {
+        const int end_live = __ldg(live);
+        for (int j = t; j < topk; j += TPR) {
+            const int to = __ldg(position + row * topk + j);
+            if (to >= 0 && to < rows * topk) scales[to] = to < end_live ? scale : 0.0f;
+        }
+    } else if (t == 0) {
+        scales[row] = scale;
+    }
+}
+
+// One thread per 16 codes of the flat array, whichever rows they belong to.
+__global__ void __launch_bounds__(256)
+int8_dequantise_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, float* __restrict__ out, size_t values, int K) {
+    ptx::chain_point();
+    const size_t group = size_t(blockIdx.x) * 256 + threadIdx.x, first = group * 16;
+    if (first >= values) return;
+    size_t row = first / uint32_t(K);
+    int column = int(first - row * uint32_t(K));
+    float scale = __ldg(scales + row);
+    auto next = [&](int8_t c) {
+        const float v = float(c) * scale;
+        if (++column == K) {
+            column = 0;
+            ++row;
+            if (row * size_t(K) < values) scale = __ldg(scales + row);
+        }
+        return v;
+    };
+    if (first + 16 <= values) {
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(codes) + group);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float4 v;
+            v.x = next(int8_t(w[q]));
+            v.y = next(int8_t(w[q] >> 8));
+            v.z = next(int8_t(w[q] >> 16));
+            v.w = next(int8_t(w[q] >> 24));
+            reinterpret_cast<float4*>(out)[group * 4 + q] = v;
+        }
+    } else {
+        for (size_t i = first; i < values; ++i) out[i] = next(codes[i]);
+    }
+}
+
+template <typename T, bool ROUTED>
+void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, const int* position, const int* live, int topk,
+            cudaStream_t stream) {
+    auto go = [&](auto kernel, int threads, int per_block) {
+        launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads), 0, stream,
+                       static_cast<const T*>(x), codes, scales, rows, K, position, live, topk);
+    };
+    const int groups = K % 16 == 0 ? K / 16 : K / 16 + 2;       // a row that starts inside a group reaches one more
+    if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED>, 256, 8);
+    else if (groups <= 128) go(int8_quantise_kernel<T, 32, 4, ROUTED>, 256, 8);
+    else if (groups <= 256) go(int8_quantise_kernel<T, 256, 1, ROUTED>, 256, 1);
+    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED>, 256, 1);
+    else if (groups <= 1024) go(int8_quantise_kernel<T, 256, 4, ROUTED>, 256, 1);
+    else if (groups <= 2048) go(int8_quantise_kernel<T, 512, 4, ROUTED>, 512, 1);
+    else go(int8_quantise_kernel<T, 512, 0, ROUTED>, 512, 1);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+}
+
+template <bool ROUTED>
+void dispatch(const void* x, int dtype, int8_t* codes, float* scales, long long rows, int K, const int* position, const int* live,
+              int topk, cudaStream_t stream) {
+    switch (dtype) {
+        case DTYPE_BF16: return launch<__nv_bfloat16, ROUTED>(x, codes, scales, rows, K, position, live, topk, stream);
+        case DTYPE_F16: return launch<__half, ROUTED>(x, codes, scales, rows, K, position, live, topk, stream);
+        case DTYPE_F32: return launch<float, ROUTED>(x, codes, scales, rows, K, position, live, topk, stream);
+        default: throw std::invalid_argument("int8: dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)");
+    }
+}
+
+void check_rows(long long rows, int K) {
+    if (rows < 0 || rows > 0x7FFFFFFFll || K < 1) throw std::invalid_argument("int8 quantise: rows must be 0..2^31-1 and K positive");
+}
+
+}  // namespace
+
+void int8_quantise(const void* x, int dtype, int8_t* codes, float* scales, long long rows, int K, cudaStream_t stream) {
+    check_rows(rows, K);
+    if (rows == 0) return;
+    if (!x || !codes || !scales) throw std::invalid_argument("int8 quantise: null pointer");
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes)) & 15)
+        throw std::invalid_argument("int8 quantise: x and codes must be 16-byte aligned");
+    dispatch<false>(x, dtype, codes, scales, rows, K, nullptr, nullptr, 1, stream);
+}
+
+void int8_gather(const void* x, int dtype, long long tokens, int topk, int K, const int* position, const int* live, int8_t* codes,
+                 float* scales, cudaStream_t stream) {
+    check_rows(tokens, K);
+    if (topk < 1 || tokens * topk > 0x7FFFFFFFll) throw std::invalid_argument("int8 gather: topk must be positive and tokens * topk below 2^31");
+    if (K % 16) throw std::invalid_argument("int8 gather: K must be a multiple of 16 (as the product of the rows wants it)");
+    if (tokens == 0) return;
+    if (!x || !codes || !scales || !position || !live) throw std::invalid_argument("int8 gather: null pointer");
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes)) & 15)
+        throw std::invalid_argument("int8 gather: x and codes must be 16-byte aligned");
+    dispatch<true>(x, dtype, codes, scales, tokens, K, position, live, topk, stream);
+}
+
+void int8_dequantise(const int8_t* codes, const float* scales, float* out, long long rows, int K, cudaStream_t stream) {
+    check_rows(rows, K);
+    if (rows == 0) return;
+    if (!codes || !scales || !out) throw std::invalid_argument("int8 dequantise: null pointer");
+    if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)
+        throw std::invalid_argument("int8 dequantise: codes and out must be 16-byte aligned");
+    const size_t values = size_t(rows) * K, blocks = (values + 4095) / 4096;
+    if (blocks > 0x7FFFFFFFull) throw std::invalid_argument("int8 dequantise: too many values");
+    launch_chained(int8_dequantise_kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, codes, scales, out, values, K);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+}
+
+}  // namespace nvfp4_b200

@@ -201,6 +201,10 @@ unsigned char* static_stage_base() {
 
 }  // namespace
 
+namespace nvfp4_b200 {
+void set_last_error(const char* message) { t_error = message; }
+}
+
 extern "C" {
 
 const char* gpu_kernels_nvfp4_last_error(void) { return t_error.c_str(); }

@@ -18,7 +18,7 @@
 // Replaces the reference's kernels/gemm/matmul/sm100.cu (prepare/launch/validate
 // at :701-737, kernel at :393-529) behind the same C++ interface.
 #include "nvfp4.h"
-#include "nvfp4_internal.h"
+#include "operators_internal.h"
 #include "ptx.cuh"
 #include "quant_device.cuh"
 
@@ -1615,6 +1615,14 @@ void validate_slot(int device, int slot) {
 }  // namespace
 
 uint32_t* device_status_word(int device) { return status_slot(device, 0); }
+
+CUtensorMap byte_rows_map(const void* p, size_t rows, size_t row_bytes, int box_rows) {
+    const cuuint64_t shape[2] = {cuuint64_t(row_bytes), cuuint64_t(rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(row_bytes)};
+    const cuuint32_t box[2] = {ROW_BYTES, cuuint32_t(box_rows)};
+    return make_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, p, 2, shape, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
 
 void require_sm100() {
     int device = 0, major = 0;

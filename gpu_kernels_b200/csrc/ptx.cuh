@@ -344,6 +344,22 @@ __device__ __forceinline__ void mma_block_scaled(uint32_t d_tmem, uint32_t a_lo,
 }
 #undef NVFP4_B200_MMA
 
+// D[tmem] (+)= A x B^T, signed 8-bit operands from shared memory, 32-bit integer sums, K = 32 per instruction; descriptors
+// as halves, as above.
+#define NVFP4_B200_MMA_I8(GROUP)                                                                                         \
+    asm volatile(                                                                                                        \
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                                  \
+        "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"                                   \
+        "tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], da, db, %4, p;\n\t}"                                           \
+        :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory")
+template <int CG>
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+    if constexpr (CG == 1) NVFP4_B200_MMA_I8("1");
+    else NVFP4_B200_MMA_I8("2");
+}
+#undef NVFP4_B200_MMA_I8
+
 // Arrive on `bar` once all tcgen05 operations issued so far by this thread have
 // completed. For a pair the arrival is delivered to the same barrier offset in
 // both CTAs.

@@ -1,0 +1,177 @@
+"""Tokens to their experts' rows and back, with gradients: what stands around an expert layer's products.
+
+A router gives each token topk experts (`route`); a route is one of these choices. `sort_routes` orders the routes by
+expert, `gather_tokens` copies the tokens' rows into that order (`gather_tokens_int8` quantises them on the way),
+`combine_tokens` adds the experts' rows up again, weighted, token by token. Both copies have gradients; the order is
+stable and every sum is taken in the order of the routes, so results do not change from run to run. The work is done by
+csrc/tokens.cu and csrc/int8_quant.cu through the C ABI (include/operators_capi.h); CPU tensors are rejected. Everything
+is asynchronous on the current stream and may be captured into a CUDA graph; nothing reads the routes back to the host.
+(Capture a backward pass with leaves that no graph outside the capture still refers to: autograd accumulates into a leaf
+on the stream where it was first used.)
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .int8 import aligned
+from .nvfp4 import _DTYPES, _require_cuda
+
+
+class Routes(NamedTuple):
+    """The order of a batch's routes: offsets int32 [E + 1] (expert e's rows are [offsets[e], offsets[e + 1])), position
+    int32 [T, topk] (each route's row) and source int32 [T * topk] (each row's route, token * topk + choice). Routes of no
+    expert have the rows from offsets[E] on."""
+    offsets: torch.Tensor
+    position: torch.Tensor
+    source: torch.Tensor
+
+
+def sort_routes(ids: torch.Tensor, num_experts: int) -> Routes:
+    """ids [T, topk] (int64 or int32): the experts each token goes to. Rows are ordered by expert and, inside an expert, by
+    token; an id outside [0, num_experts) (a router's "dropped" mark such as -1) belongs to no expert. Up to 1024 experts."""
+    _require_cuda(ids, "ids")
+    if ids.dim() != 2 or ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError("ids must be an int64 or int32 tensor [tokens, topk]")
+    if not 1 <= num_experts <= 1024:
+        raise ValueError("1..1024 experts")
+    ids = ids.contiguous()
+    routes, d = ids.numel(), ids.device
+    if routes >= 1 << 31:
+        raise ValueError("fewer than 2^31 routes")
+    offsets = torch.empty((num_experts + 1,), dtype=torch.int32, device=d)
+    position = torch.empty(ids.shape, dtype=torch.int32, device=d)
+    source = torch.empty((routes,), dtype=torch.int32, device=d)
+    with _lib.on(d):
+        _lib.check(_lib.load().gpu_kernels_tokens_sort(
+            ids.data_ptr(), ids.element_size(), routes, num_experts, offsets.data_ptr(), position.data_ptr(), source.data_ptr(),
+            _lib.stream()))
+    return Routes(offsets, position, source)
+
+
+def _check_routes(routes: Routes, tokens: int | None, device) -> tuple[int, int, int, int]:
+    """(position, live rows, tokens, topk) of a checked order, the first two as device addresses."""
+    offsets, position = routes.offsets, routes.position
+    if position.dim() != 2 or position.shape[1] < 1 or (tokens is not None and position.shape[0] != tokens):
+        raise ValueError("the routes are not those of this many tokens")
+    for name, t in (("offsets", offsets), ("position", position)):
+        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError(f"routes.{name} must be a contiguous int32 tensor on {device}")
+    if offsets.dim() != 1 or offsets.numel() < 2:
+        raise ValueError("routes.offsets must hold one value per expert and one more")
+    return position.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), position.shape[0], position.shape[1]
+
+
+def _values(t: torch.Tensor, name: str) -> torch.Tensor:
+    _require_cuda(t, name)
+    if t.dim() != 2 or t.dtype not in _DTYPES or t.shape[1] < 1:
+        raise ValueError(f"{name} must be a bf16, fp16 or fp32 tensor [rows, hidden]")
+    return t
+
+
+def _gather(x, routes):
+    x = x.contiguous()
+    position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
+    rows = torch.empty((tokens * topk, x.shape[1]), dtype=x.dtype, device=x.device)
+    with _lib.on(x.device):
+        _lib.check(_lib.load().gpu_kernels_tokens_gather(
+            x.data_ptr(), _DTYPES[x.dtype], tokens, topk, x.shape[1], position, live, rows.data_ptr(), _lib.stream()))
+    return rows
+
+
+def _combine(rows, routes, weights):
+    rows = rows.contiguous()
+    position, live, tokens, topk = _check_routes(routes, None, rows.device)
+    y = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    with _lib.on(rows.device):
+        _lib.check(_lib.load().gpu_kernels_tokens_combine(
+            rows.data_ptr(), _DTYPES[rows.dtype], None if weights is None else weights.data_ptr(), position, live, tokens, topk,
+            rows.shape[1], y.data_ptr(), _lib.stream()))
+    return y
+
+
+class _GatherTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, routes):
+        ctx.save_for_backward(*routes)
+        return _gather(x, routes)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_rows):
+        return _combine(d_rows, Routes(*ctx.saved_tensors), None), None
+
+
+class _CombineTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, routes):
+        ctx.save_for_backward(rows if weights is not None and ctx.needs_input_grad[1] else None, weights, *routes)
+        return _combine(rows, routes, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_y):
+        rows, weights, *order = ctx.saved_tensors
+        routes = Routes(*order)
+        if weights is None:
+            return _gather(d_y, routes), None, None
+        d_y = d_y.contiguous()
+        position, live, tokens, topk = _check_routes(routes, d_y.shape[0], d_y.device)
+        d_rows = d_weights = None
+        if ctx.needs_input_grad[0]:
+            d_rows = torch.empty((tokens * topk, d_y.shape[1]), dtype=d_y.dtype, device=d_y.device)
+        if ctx.needs_input_grad[1]:
+            d_weights = torch.empty((tokens, topk), dtype=torch.float32, device=d_y.device)
+            rows = rows.contiguous()
+        with _lib.on(d_y.device):
+            _lib.check(_lib.load().gpu_kernels_tokens_combine_backward(
+                d_y.data_ptr(), _DTYPES[d_y.dtype], None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live,
+                tokens, topk, d_y.shape[1], None if d_rows is None else d_rows.data_ptr(),
+                None if d_weights is None else d_weights.data_ptr(), _lib.stream()))
+        return d_rows, d_weights, None
+
+
+def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
+    """x [T, H] -> rows [T * topk, H]: each route's row is its token's. Rows of no expert are zeros.
+
+    Gradient: x's is the sum of its live rows' gradients, in FP32 and the order of the routes, rounded once."""
+    _values(x, "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _GatherTokens.apply(x, routes)
+    return _gather(x, routes)
+
+
+def gather_tokens_int8(x: torch.Tensor, routes: Routes):
+    """quantize_int8(x) in the order of the routes: x [T, K] -> (codes int8 [T * topk, K], scales fp32 [T * topk]), the rows
+    `int8_grouped_gemm` takes. A token is quantised once, K a multiple of 16; rows of no expert have codes and scale 0."""
+    x = aligned(_values(x, "x").detach())
+    position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
+    k = x.shape[1]
+    if k % 16:
+        raise ValueError("K must be a multiple of 16")
+    codes = torch.empty((tokens * topk, k), dtype=torch.int8, device=x.device)
+    scales = torch.empty((tokens * topk,), dtype=torch.float32, device=x.device)
+    with _lib.on(x.device):
+        _lib.check(_lib.load().gpu_kernels_tokens_gather_int8(
+            x.data_ptr(), _DTYPES[x.dtype], tokens, topk, k, position, live, codes.data_ptr(), scales.data_ptr(), _lib.stream()))
+    return codes, scales
+
+
+def combine_tokens(rows: torch.Tensor, routes: Routes, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """rows [T * topk, H], weights [T, topk] -> y [T, H]: the sum over a token's live routes of weight * row (None: of the
+    rows), in FP32 and the order of the routes, rounded once. Rows of no expert are not read, whatever they hold.
+
+    Gradients: a live row's is weight * d_y of its token, a weight's is <d_y, row>; zero for routes of no expert."""
+    _values(rows, "rows")
+    if rows.shape[0] != routes.position.numel():
+        raise ValueError("the routes are not those of this many rows")
+    if weights is not None:
+        if weights.shape != routes.position.shape or weights.device != rows.device or not weights.is_floating_point():
+            raise ValueError("weights must be floating-point, [tokens, topk] and where the rows are")
+        weights = weights.float().contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _CombineTokens.apply(rows, weights, routes)
+    return _combine(rows, routes, weights)
