@@ -87,7 +87,8 @@ OPERATOR_SIGNATURES = {
     "gpu_kernels_int8_linear": ([P, I, P, P, P, P, P, I, I, I, I, P], I),
     "gpu_kernels_int8_grouped_gemm": ([P, P, P, P, P, I, P, I, I, I, I, I, P], I),
     "gpu_kernels_int8_tiles": ([I, I, I, I, ctypes.POINTER(I)], I),
-    "gpu_kernels_tokens_sort": ([P, I, I, I, P, P, P, P], I),
+    "gpu_kernels_tokens_sort": ([P, I, I, I, P, P, P, P, P], I),
+    "gpu_kernels_tokens_sort_workspace": ([I, I], ctypes.c_size_t),
     "gpu_kernels_tokens_gather": ([P, I, I, I, I, P, P, P, P], I),
     "gpu_kernels_tokens_gather_int8": ([P, I, I, I, I, P, P, P, P, P], I),
     "gpu_kernels_tokens_combine": ([P, I, P, P, P, I, I, I, P, P], I),

@@ -81,11 +81,15 @@ int gpu_kernels_int8_tiles(int rows, int N, int K, int experts, int* info) {
     });
 }
 
+size_t gpu_kernels_tokens_sort_workspace(int routes, int experts) {
+    return routes < 0 || experts < 1 ? 0 : tokens_sort_workspace(routes, experts);
+}
+
 int gpu_kernels_tokens_sort(const void* ids, int id_bytes, int routes, int experts, void* offsets, void* position, void* source,
-                            void* stream) {
+                            void* workspace, void* stream) {
     return guarded([&] {
         tokens_sort(ids, id_bytes, routes, experts, static_cast<int*>(offsets), static_cast<int*>(position), static_cast<int*>(source),
-                    on(stream));
+                    static_cast<int*>(workspace), on(stream));
     });
 }
 

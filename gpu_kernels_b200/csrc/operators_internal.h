@@ -45,7 +45,9 @@ void int8_grouped_gemm(const int8_t* rows, const int8_t* weights, const float* r
                        cudaStream_t stream);
 
 // tokens.cu
-void tokens_sort(const void* ids, int id_bytes, int routes, int experts, int* offsets, int* position, int* source, cudaStream_t stream);
+void tokens_sort(const void* ids, int id_bytes, int routes, int experts, int* offsets, int* position, int* source, int* workspace,
+                 cudaStream_t stream);
+size_t tokens_sort_workspace(int routes, int experts);
 void tokens_gather(const void* x, int dtype, int tokens, int topk, int hidden, const int* position, const int* live, void* rows,
                    cudaStream_t stream);
 void tokens_combine(const void* rows, int dtype, const float* weights, const int* position, const int* live, int tokens, int topk,

@@ -13,105 +13,144 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 
 namespace nvfp4_b200 {
 namespace {
 
 // ---- the order ------------------------------------------------------------------------------------------------------
-// A counting sort in one launch of one cluster. The routes are cut into one contiguous part per warp of the cluster; a
-// warp counts its part in a row of counters of its own, 32 routes at a time (lanes with the same expert find each other
-// by __match_any_sync, the lowest of them adds their number), so no atomics are needed and the order is stable. Sums
-// over the warps and, through distributed shared memory, over the CTAs give each (warp, expert) its first row; a second
-// walk over the same routes hands the rows out. The bytes are nothing (1 MB at 131072 routes): latency is the bound.
+// A stable counting sort. The bytes are nothing (2 MB at 131072 routes); latency is the bound, and on few SMs the 4-byte
+// stores of `source`, each in a sector of its own: as one cluster of eight CTAs 131072 routes took 32 us, on 128 CTAs 11.
+// Three forms: up to SMALL routes every route is compared with every other; up to one block's worth (BLOCK) one CTA
+// counts and hands out rows; beyond, a first launch counts each block's routes and a second one, with a CTA for each of
+// the same blocks, adds up the counts of the blocks before its own.
 constexpr int SORT_MAX_EXPERTS = 1024;
+constexpr int SMALL = 256, BLOCK = 1024, SORT_WARPS = BLOCK / 32;
 
-template <typename Id, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-tokens_sort_kernel(const Id* __restrict__ ids, int routes, int experts, int* __restrict__ offsets, int* __restrict__ position,
-                   int* __restrict__ source) {
+template <typename Id>
+__device__ __forceinline__ int key_of(const Id* ids, long long i, int experts) {
+    const long long id = (long long)(__ldg(ids + i));
+    return id >= 0 && id < experts ? int(id) : experts;         // `experts`: dropped
+}
+
+// A route's row is the number of routes with a smaller key, or with the same key in front of it; an expert's first row is
+// the number of routes with a smaller key.
+template <typename Id>
+__global__ void __launch_bounds__(SMALL)
+tokens_sort_small_kernel(const Id* __restrict__ ids, int routes, int experts, int* __restrict__ offsets, int* __restrict__ position,
+                         int* __restrict__ source) {
     ptx::chain_point();
-    constexpr int WARPS = THREADS / 32;
-    const int keys = experts + 1;                               // the last one: dropped
-    extern __shared__ int counters[];                           // [WARPS][keys], then the CTA's totals and first rows [keys] each
-    int* totals = counters + WARPS * keys;
-    int* first = totals + keys;
-    __shared__ int warp_sum[WARPS];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    uint32_t ctas;
-    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
-    const uint32_t rank = ptx::cluster_ctarank();
-    for (int i = threadIdx.x; i < WARPS * keys; i += THREADS) counters[i] = 0;
+    __shared__ __align__(16) int keys[SMALL];
+    const int i = threadIdx.x, own = i < routes ? key_of(ids, i, experts) : INT_MAX;
+    keys[i] = own;
     __syncthreads();
-    const long long parts = (long long)(ctas) * WARPS;
-    const long long part = ((routes + parts - 1) / parts + 31) / 32 * 32;
-    const long long begin = (long long)(rank * WARPS + warp) * part;
-    const int steps = begin < routes ? int((min((long long)(routes), begin + part) - begin + 31) / 32) : 0;
+    const int4* four = reinterpret_cast<const int4*>(keys);
+    const int fours = (routes + 3) / 4;
+    int row = 0;
+    #pragma unroll 4
+    for (int j = 0; j < fours; ++j) {
+        const int4 k = four[j];
+        row += (k.x < own || (k.x == own && 4 * j < i)) + (k.y < own || (k.y == own && 4 * j + 1 < i)) +
+               (k.z < own || (k.z == own && 4 * j + 2 < i)) + (k.w < own || (k.w == own && 4 * j + 3 < i));
+    }
+    if (i < routes) {
+        position[i] = row;
+        source[row] = i;
+    }
+    for (int e = i; e <= experts; e += SMALL) {
+        int first = 0;
+        #pragma unroll 4
+        for (int j = 0; j < fours; ++j) {
+            const int4 k = four[j];
+            first += (k.x < e) + (k.y < e) + (k.z < e) + (k.w < e);
+        }
+        offsets[e] = first;
+    }
+}
+
+// counts[block][key]: the routes of each key (dropped ones last) in a block of `part` routes.
+template <typename Id>
+__global__ void __launch_bounds__(BLOCK)
+tokens_count_kernel(const Id* __restrict__ ids, int routes, int experts, int part, int* __restrict__ counts) {
+    ptx::chain_point();
+    extern __shared__ int count[];
+    for (int e = threadIdx.x; e <= experts; e += BLOCK) count[e] = 0;
+    __syncthreads();
+    const long long begin = (long long)(blockIdx.x) * part, end = min((long long)(routes), begin + part);
+    for (long long i = begin + threadIdx.x; i < end; i += BLOCK) atomicAdd(&count[key_of(ids, i, experts)], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e <= experts; e += BLOCK) counts[size_t(blockIdx.x) * (experts + 1) + e] = count[e];
+}
+
+// A warp counts a contiguous part of its block's routes in a row of counters of its own, 32 routes at a time: lanes with
+// the same expert find each other by one ballot per bit of the key, the lowest of them adds their number, so no atomics
+// are needed and the order is stable. Sums over the warps and the blocks before give each (warp, expert) its first row; a
+// second walk over the same routes hands the rows out.
+template <typename Id>
+__global__ void __launch_bounds__(BLOCK)
+tokens_sort_kernel(const Id* __restrict__ ids, int routes, int experts, int part, const int* __restrict__ counts,
+                   int* __restrict__ offsets, int* __restrict__ position, int* __restrict__ source) {
+    ptx::chain_point();
+    const int keys = experts + 1, bits = 32 - __clz(experts);
+    extern __shared__ int counters[];                           // [SORT_WARPS][keys], then for each key, [keys] each:
+    int* first = counters + SORT_WARPS * keys;                  // its routes in the blocks before, later its first row in this block
+    int* others = first + keys;                                 // its routes in the other blocks
+    __shared__ int warp_sum[SORT_WARPS];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int i = threadIdx.x; i < (SORT_WARPS + 2) * keys; i += BLOCK) counters[i] = 0;
+    __syncthreads();
+    if (counts) {
+        const int all = int(gridDim.x) * keys, mine = int(blockIdx.x) * keys;
+        #pragma unroll 8
+        for (int i = threadIdx.x; i < all; i += BLOCK) {
+            const int n = __ldcg(counts + i), e = i % keys;
+            if (n == 0) continue;
+            if (i < mine) atomicAdd(first + e, n);
+            if (i < mine || i >= mine + keys) atomicAdd(others + e, n);
+        }
+    }
+    const int per_warp = part / SORT_WARPS;                     // a multiple of 32
+    const long long begin = (long long)(blockIdx.x) * part + warp * per_warp;
+    const int steps = begin < routes ? int((min((long long)(routes), begin + per_warp) - begin + 31) / 32) : 0;
     int* own = counters + warp * keys;
-    auto key_of = [&](int step) {
-        const long long i = begin + step * 32 + lane;
-        if (step >= steps || i >= routes) return -1;            // no route: matches only its own kind
-        const long long id = (long long)(__ldg(ids + i));
-        return id >= 0 && id < experts ? int(id) : experts;
-    };
-    // The keys of four steps are loaded ahead of the four that are counted.
     auto walk = [&](auto&& body) {
-        int ahead[4];
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) ahead[j] = key_of(j);
-        for (int step = 0; step < steps; step += 4) {
-            int now[4];
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) { now[j] = ahead[j]; ahead[j] = key_of(step + 4 + j); }
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t peers = __match_any_sync(0xFFFFFFFFu, now[j]);
-                body(step + j, now[j], peers);
-                __syncwarp();
+        auto key = [&](int step) {
+            const long long i = begin + step * 32 + lane;
+            return step < steps && i < routes ? key_of(ids, i, experts) : -1;
+        };
+        int next = key(0);
+        for (int step = 0; step < steps; ++step) {
+            const int now = next;
+            next = key(step + 1);
+            uint32_t peers = __ballot_sync(0xFFFFFFFFu, now >= 0);
+            for (int b = 0; b < bits; ++b) {
+                const bool set = (now >> b) & 1;
+                const uint32_t same = __ballot_sync(0xFFFFFFFFu, set);
+                peers &= set ? same : ~same;
             }
+            body(step, now, peers);
+            __syncwarp();
         }
     };
     walk([&](int, int key, uint32_t peers) {
         if (key >= 0 && lane == __ffs(peers) - 1) own[key] += __popc(peers);
     });
     __syncthreads();
-    for (int e = threadIdx.x; e < keys; e += THREADS) {         // counts -> routes of the same expert in the warps before
-        int sum = 0;
-        #pragma unroll 8
-        for (int w = 0; w < WARPS; ++w) {
-            const int c = counters[w * keys + e];
-            counters[w * keys + e] = sum;
-            sum += c;
-        }
-        totals[e] = sum;
-    }
-    __syncwarp();
-    ptx::cluster_arrive();
-    ptx::cluster_wait();
-    // Every CTA: the routes of each expert in the whole cluster and in the CTAs before it, and the sum of the former over
-    // the experts before, a run of consecutive experts per thread.
-    const int run = (experts + THREADS - 1) / THREADS, e0 = min(experts, int(threadIdx.x) * run), e1 = min(experts, e0 + run);
+    // A run of consecutive keys per thread: the routes of each in all blocks, and the first row of each in this block (in
+    // front of it: the smaller keys of all blocks, the same key of the blocks before).
+    const int run = (keys + BLOCK - 1) / BLOCK, e0 = min(keys, int(threadIdx.x) * run), e1 = min(keys, e0 + run);
     int sum = 0;
     for (int e = e0; e < e1; ++e) {
-        int all = 0, before = 0;
-        for (uint32_t c = 0; c < ctas; ++c) {
-            int n;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(ptx::map_to_cta(ptx::smem_u32(totals + e), c)) : "memory");
-            before += c < rank ? n : 0;
-            all += n;
+        int here = 0;
+        #pragma unroll 8
+        for (int w = 0; w < SORT_WARPS; ++w) {
+            const int c = counters[w * keys + e];
+            counters[w * keys + e] = here;
+            here += c;
         }
-        first[e] = sum + before;                                // still without the experts of the threads before
-        sum += all;
+        first[e] += sum;                                        // still without the keys of the threads before
+        sum += here + others[e];
     }
-    int dropped_before = 0;
-    if (threadIdx.x == 0) {
-        for (uint32_t c = 0; c < rank; ++c) {
-            int n;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(ptx::map_to_cta(ptx::smem_u32(totals + experts), c)) : "memory");
-            dropped_before += n;
-        }
-    }
-    __syncwarp();
-    ptx::cluster_arrive();                                      // (waited for at the end: the others may still be reading)
     int upto = sum;                                             // inclusive over the warp
     #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -120,23 +159,16 @@ tokens_sort_kernel(const Id* __restrict__ ids, int routes, int experts, int* __r
     }
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
-    int start = upto - sum, total = 0;
+    int start = upto - sum;
     #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        const int n = warp_sum[w];
-        start += w < warp ? n : 0;
-        total += n;
+    for (int w = 0; w < SORT_WARPS; ++w) start += w < warp ? warp_sum[w] : 0;
+    for (int e = e0; e < e1; ++e) {
+        first[e] += start;
+        if (blockIdx.x == 0) offsets[e] = first[e];             // (no block before the first)
     }
-    // offsets[e] is the first row of e over all CTAs; this CTA's first row lies behind those of the CTAs before it
-    if (rank == 0) {
-        for (int e = e0; e < e1; ++e) offsets[e] = start + first[e];
-        if (threadIdx.x == 0) offsets[experts] = total;
-    }
-    for (int e = e0; e < e1; ++e) first[e] += start;
-    if (threadIdx.x == 0) first[experts] = total + dropped_before;
     __syncthreads();
     walk([&](int step, int key, uint32_t peers) {
-        const int leader = __ffs(peers) - 1;
+        const int leader = key >= 0 ? __ffs(peers) - 1 : lane;
         int row = 0;
         if (key >= 0 && lane == leader) {
             row = first[key] + own[key];
@@ -150,125 +182,194 @@ tokens_sort_kernel(const Id* __restrict__ ids, int routes, int experts, int* __r
             source[row] = int(i);
         }
     });
-    __syncwarp();
-    ptx::cluster_wait();
+}
+
+// Blocks of the larger form, and the routes of each (a multiple of BLOCK).
+int sort_blocks(int routes, int& part) {
+    constexpr int MOST = 64;
+    part = int((((long long)(routes) + MOST - 1) / MOST + BLOCK - 1) / BLOCK * BLOCK);
+    return int(((long long)(routes) + part - 1) / part);
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------------
 
-template <typename T> __device__ __forceinline__ float widen(T v);
-template <> __device__ __forceinline__ float widen(float v) { return v; }
-template <> __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
-
-// N values of T, loaded and stored at once: 16 bytes, or one value where rows do not start on 16-byte boundaries.
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-    T v[N];
+template <typename T> struct Format;                            // one 32-bit word as FP32 values, and back
+template <> struct Format<float> {
+    static __device__ __forceinline__ float get(uint32_t w, int) { return __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t put(float a, float) { return __float_as_uint(a); }
 };
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load(const T* p) {
-    if constexpr (sizeof(T) * N == 16) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
-        return *reinterpret_cast<const Pack<T, N>*>(&raw);
-    } else {
-        return *reinterpret_cast<const Pack<T, N>*>(p);
+template <> struct Format<__nv_bfloat16> {
+    static __device__ __forceinline__ float get(uint32_t w, int i) { return __uint_as_float(i ? w & 0xFFFF0000u : w << 16); }
+    static __device__ __forceinline__ uint32_t put(float a, float b) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&p);
     }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const Pack<T, N>& v) {
-    if constexpr (sizeof(T) * N == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&v);
-    else *reinterpret_cast<Pack<T, N>*>(p) = v;
-}
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> zeros() {
-    Pack<T, N> z;
-    #pragma unroll
-    for (int i = 0; i < N; ++i) z.v[i] = narrow<T>(0.0f);
-    return z;
-}
+};
+template <> struct Format<__half> {
+    static __device__ __forceinline__ float get(uint32_t w, int i) { return __half2float(__ushort_as_half(static_cast<unsigned short>(i ? w >> 16 : w))); }
+    static __device__ __forceinline__ uint32_t put(float a, float b) {
+        const __half2 p = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&p);
+    }
+};
 
+// N values of T that are loaded and stored at once: 16 bytes, or as many as divide a row where rows do not start on
+// 16-byte boundaries.
+template <typename T, int N>
+struct Pack {
+    static constexpr int BYTES = int(sizeof(T)) * N, WORDS = BYTES < 4 ? 1 : BYTES / 4, PER_WORD = 4 / int(sizeof(T));
+    using Word = typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2,
+                 typename std::conditional<BYTES == 4, uint32_t, unsigned short>::type>::type>::type;
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void load(const T* p) {
+        const Word v = __ldg(reinterpret_cast<const Word*>(p));
+        if constexpr (BYTES == 16) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+        else if constexpr (BYTES == 8) { w[0] = v.x; w[1] = v.y; }
+        else w[0] = v;
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (BYTES == 16) *reinterpret_cast<Word*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (BYTES == 8) *reinterpret_cast<Word*>(p) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<Word*>(p) = Word(w[0]);
+    }
+    __device__ __forceinline__ float operator[](int i) const { return Format<T>::get(w[i / PER_WORD], i % PER_WORD); }
+    __device__ __forceinline__ void set(const float (&v)[N]) {
+        #pragma unroll
+        for (int i = 0; i < N; i += PER_WORD) w[i / PER_WORD] = Format<T>::put(v[i], i + 1 < N ? v[i + 1] : 0.0f);
+    }
+    __device__ __forceinline__ void clear() {
+        #pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+    }
+};
+
+// A block of ROW_THREADS threads per token and segment of its row. A segment is one pack per thread or two, and eight of
+// fewer than 16 bytes, whose blocks would be over before they have begun.
 constexpr int ROW_THREADS = 128;
-constexpr int GATHER_PACKS = 2;                                 // packs of a row per thread
+constexpr int NARROW = 8;
+template <typename T, int N> constexpr int GATHER_PACKS = sizeof(T) * N == 16 ? 2 : NARROW;
 
-// rows[position[t, j]] = x[t] for every route j of token t: the token's row is read once. One block per token and
-// segment of the row.
+// rows[position[t, j]] = x[t] for every route j of token t: the token's row is read once.
 template <typename T, int N>
 __global__ void __launch_bounds__(ROW_THREADS)
 tokens_gather_kernel(const T* __restrict__ x, T* __restrict__ rows, const int* __restrict__ position, const int* __restrict__ live,
                      int tokens, int topk, int hidden, int segments) {
     ptx::chain_point();
+    constexpr int PACKS = GATHER_PACKS<T, N>;
     const int token = blockIdx.x / segments, packs = hidden / N;
-    const int p0 = (blockIdx.x - token * segments) * (ROW_THREADS * GATHER_PACKS) + threadIdx.x;
-    Pack<T, N> v[GATHER_PACKS];
+    const int p0 = (blockIdx.x - token * segments) * (ROW_THREADS * PACKS) + threadIdx.x;
+    Pack<T, N> v[PACKS];
     #pragma unroll
-    for (int u = 0; u < GATHER_PACKS; ++u)
-        if (p0 + u * ROW_THREADS < packs) v[u] = load<T, N>(x + size_t(token) * hidden + size_t(p0 + u * ROW_THREADS) * N);
+    for (int u = 0; u < PACKS; ++u)
+        if (p0 + u * ROW_THREADS < packs) v[u].load(x + size_t(token) * hidden + size_t(p0 + u * ROW_THREADS) * N);
     const int end_live = __ldg(live);
     for (int j = 0; j < topk; ++j) {
         const int to = __ldg(position + size_t(token) * topk + j);
         if (to < 0 || to >= tokens * topk) continue;
+        T* row = rows + size_t(to) * hidden;
         #pragma unroll
-        for (int u = 0; u < GATHER_PACKS; ++u)
-            if (p0 + u * ROW_THREADS < packs)
-                store<T, N>(rows + size_t(to) * hidden + size_t(p0 + u * ROW_THREADS) * N, to < end_live ? v[u] : zeros<T, N>());
+        for (int u = 0; u < PACKS; ++u) {
+            if (p0 + u * ROW_THREADS >= packs) continue;
+            Pack<T, N> out = v[u];
+            if (to >= end_live) out.clear();
+            out.store(row + size_t(p0 + u * ROW_THREADS) * N);
+        }
     }
 }
 
 // y[t] = sum over the live routes j of token t, in their order, of weights[t, j] * rows[position[t, j]] (weights null: of
-// the rows as they are, which is the gradient of the gather): FP32 sums, rounded once. Up to eight rows are in flight.
-template <typename T, int N, bool WEIGHTED>
+// the rows as they are, which is the gradient of the gather): FP32 sums, rounded once. GROUP rows are in flight at a time;
+// as few as topk needs, since registers are what bounds the loads in flight (4096 tokens of 4096 bf16 values, topk 6: with
+// room for eight 44 us, for six 41).
+template <typename T, int GROUP>
 __global__ void __launch_bounds__(ROW_THREADS)
 tokens_combine_kernel(const T* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ position,
                       const int* __restrict__ live, int tokens, int topk, int hidden, int segments, T* __restrict__ y) {
     ptx::chain_point();
-    constexpr int AHEAD = 8;
-    const int token = blockIdx.x / segments, packs = hidden / N;
+    constexpr int N = 16 / int(sizeof(T));
+    const int token = blockIdx.x / segments;
     const int p = (blockIdx.x - token * segments) * ROW_THREADS + threadIdx.x;
-    if (p >= packs) return;
+    if (p >= hidden / N) return;
     const int end_live = min(__ldg(live), tokens * topk);
     float sum[N];
     #pragma unroll
     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-    for (int j0 = 0; j0 < topk; j0 += AHEAD) {
-        Pack<T, N> v[AHEAD];
-        int from[AHEAD];
+    for (int j0 = 0; j0 < topk; j0 += GROUP) {
+        Pack<T, N> v[GROUP];
+        bool there[GROUP];
         #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            from[j] = j0 + j < topk ? __ldg(position + size_t(token) * topk + j0 + j) : -1;
-            if (from[j] >= end_live) from[j] = -1;
-            if (from[j] >= 0) v[j] = load<T, N>(rows + size_t(from[j]) * hidden + size_t(p) * N);
+        for (int j = 0; j < GROUP; ++j) {
+            const int from = j0 + j < topk ? __ldg(position + size_t(token) * topk + j0 + j) : -1;
+            there[j] = from >= 0 && from < end_live;
+            if (there[j]) v[j].load(rows + size_t(from) * hidden + size_t(p) * N);
         }
         #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            if (from[j] < 0) continue;
-            const float w = WEIGHTED ? __ldg(weights + size_t(token) * topk + j0 + j) : 1.0f;
+        for (int j = 0; j < GROUP; ++j) {
+            if (!there[j]) continue;
+            const float w = weights ? __ldg(weights + size_t(token) * topk + j0 + j) : 1.0f;
             #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] = WEIGHTED ? __fmaf_rn(w, widen(v[j].v[i]), sum[i]) : sum[i] + widen(v[j].v[i]);
+            for (int i = 0; i < N; ++i) sum[i] = __fmaf_rn(w, v[j][i], sum[i]);
         }
     }
     Pack<T, N> out;
+    out.set(sum);
+    out.store(y + size_t(token) * hidden + size_t(p) * N);
+}
+
+// The same for rows of narrower packs (an odd number of values, say): eight packs of one row in flight per thread instead
+// of one pack of several rows, so that what surrounds a load is paid once for eight (1000 tokens of 2975 bf16 values, topk
+// 2: pack by pack 20.7 us).
+template <typename T, int N>
+__global__ void __launch_bounds__(ROW_THREADS)
+tokens_combine_narrow_kernel(const T* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ position,
+                             const int* __restrict__ live, int tokens, int topk, int hidden, int segments, T* __restrict__ y) {
+    ptx::chain_point();
+    const int token = blockIdx.x / segments, packs = hidden / N;
+    const int p0 = (blockIdx.x - token * segments) * (ROW_THREADS * NARROW) + threadIdx.x;
+    const int end_live = min(__ldg(live), tokens * topk);
+    float sum[NARROW][N];
     #pragma unroll
-    for (int i = 0; i < N; ++i) out.v[i] = narrow<T>(sum[i]);
-    store<T, N>(y + size_t(token) * hidden + size_t(p) * N, out);
+    for (int u = 0; u < NARROW; ++u)
+        #pragma unroll
+        for (int i = 0; i < N; ++i) sum[u][i] = 0.0f;
+    for (int j = 0; j < topk; ++j) {
+        const int from = __ldg(position + size_t(token) * topk + j);
+        if (from < 0 || from >= end_live) continue;
+        const float w = weights ? __ldg(weights + size_t(token) * topk + j) : 1.0f;
+        const T* row = rows + size_t(from) * hidden;
+        Pack<T, N> v[NARROW];
+        #pragma unroll
+        for (int u = 0; u < NARROW; ++u)
+            if (p0 + u * ROW_THREADS < packs) v[u].load(row + (p0 + u * ROW_THREADS) * N);
+        #pragma unroll
+        for (int u = 0; u < NARROW; ++u) {
+            if (p0 + u * ROW_THREADS >= packs) continue;
+            #pragma unroll
+            for (int i = 0; i < N; ++i) sum[u][i] = __fmaf_rn(w, v[u][i], sum[u][i]);
+        }
+    }
+    #pragma unroll
+    for (int u = 0; u < NARROW; ++u) {
+        if (p0 + u * ROW_THREADS >= packs) continue;
+        Pack<T, N> out;
+        out.set(sum[u]);
+        out.store(y + size_t(token) * hidden + (p0 + u * ROW_THREADS) * N);
+    }
 }
 
 // d_rows[position[t, j]] = weights[t, j] * d_y[t] (null: not asked for), d_weights[t, j] = <d_y[t], rows[position[t, j]]>
-// (null: not asked for, the rows are then not read). A block per token: the token's gradient is read once for eight
+// (null: not asked for, the rows are then not read). A block per token: the token's gradient is read once for GROUP
 // routes, whose sums stay in registers; lanes, then warps, are added in a fixed order.
-template <typename T, int N>
-__global__ void __launch_bounds__(256)
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(ROW_THREADS, 6)
 tokens_combine_backward_kernel(const T* __restrict__ d_y, const T* __restrict__ rows, const float* __restrict__ weights,
                                const int* __restrict__ position, const int* __restrict__ live, int tokens, int topk, int hidden,
                                T* __restrict__ d_rows, float* __restrict__ d_weights) {
     ptx::chain_point();
-    constexpr int GROUP = 8, WARPS = 8;
+    constexpr int WARPS = ROW_THREADS / 32, N = 16 / int(sizeof(T));
     __shared__ float partial[GROUP][WARPS];
-    const int token = blockIdx.x, packs = hidden / N, end_live = __ldg(live);
+    const int token = blockIdx.x, packs = hidden / N, end_live = min(__ldg(live), tokens * topk);
     for (int j0 = 0; j0 < topk; j0 += GROUP) {
         int at[GROUP];
         float w[GROUP], dot[GROUP];
@@ -279,22 +380,31 @@ tokens_combine_backward_kernel(const T* __restrict__ d_y, const T* __restrict__ 
             w[j] = at[j] >= 0 && at[j] < end_live ? __ldg(weights + size_t(token) * topk + j0 + j) : 0.0f;
             dot[j] = 0.0f;
         }
-        for (int p = threadIdx.x; p < packs; p += 256) {
-            const Pack<T, N> g = load<T, N>(d_y + size_t(token) * hidden + size_t(p) * N);
-            #pragma unroll
-            for (int j = 0; j < GROUP; ++j) {
-                if (at[j] < 0) continue;
-                const size_t place = size_t(at[j]) * hidden + size_t(p) * N;
-                if (d_weights && at[j] < end_live) {
-                    const Pack<T, N> r = load<T, N>(rows + place);
+        for (int p = threadIdx.x; p < packs; p += ROW_THREADS) {
+            Pack<T, N> g, r[GROUP];
+            g.load(d_y + size_t(token) * hidden + size_t(p) * N);
+            if (d_weights) {
+                #pragma unroll
+                for (int j = 0; j < GROUP; ++j)                 // all the loads before the first store
+                    if (at[j] >= 0 && at[j] < end_live) r[j].load(rows + size_t(at[j]) * hidden + size_t(p) * N);
+                #pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    if (at[j] < 0 || at[j] >= end_live) continue;
                     #pragma unroll
-                    for (int i = 0; i < N; ++i) dot[j] = __fmaf_rn(widen(g.v[i]), widen(r.v[i]), dot[j]);
+                    for (int i = 0; i < N; ++i) dot[j] = __fmaf_rn(g[i], r[j][i], dot[j]);
                 }
-                if (d_rows) {
-                    Pack<T, N> out;
+            }
+            if (d_rows) {
+                #pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    if (at[j] < 0) continue;
+                    float v[N];
                     #pragma unroll
-                    for (int i = 0; i < N; ++i) out.v[i] = narrow<T>(at[j] < end_live ? w[j] * widen(g.v[i]) : 0.0f);
-                    store<T, N>(d_rows + place, out);
+                    for (int i = 0; i < N; ++i) v[i] = w[j] * g[i];
+                    Pack<T, N> out;
+                    out.set(v);
+                    if (at[j] >= end_live) out.clear();
+                    out.store(d_rows + size_t(at[j]) * hidden + size_t(p) * N);
                 }
             }
         }
@@ -316,15 +426,75 @@ tokens_combine_backward_kernel(const T* __restrict__ d_y, const T* __restrict__ 
     }
 }
 
+// The same for rows of narrower packs: a route at a time, eight packs of its row in flight per thread. The token's gradient
+// comes from L1 after the first route.
+template <typename T, int N>
+__global__ void __launch_bounds__(ROW_THREADS)
+tokens_combine_backward_narrow_kernel(const T* __restrict__ d_y, const T* __restrict__ rows, const float* __restrict__ weights,
+                                      const int* __restrict__ position, const int* __restrict__ live, int tokens, int topk,
+                                      int hidden, T* __restrict__ d_rows, float* __restrict__ d_weights) {
+    ptx::chain_point();
+    constexpr int WARPS = ROW_THREADS / 32;
+    __shared__ float partial[2][WARPS];                         // (two, so that one barrier per route is enough)
+    const int token = blockIdx.x, packs = hidden / N, end_live = min(__ldg(live), tokens * topk);
+    const T* gradient = d_y + size_t(token) * hidden;
+    for (int j = 0; j < topk; ++j) {
+        const int at = __ldg(position + size_t(token) * topk + j);
+        const bool there = at >= 0 && at < tokens * topk, counts = there && at < end_live;
+        const float w = counts ? __ldg(weights + size_t(token) * topk + j) : 0.0f;
+        const size_t row = there ? size_t(at) * hidden : 0;
+        float dot = 0.0f;
+        for (int p0 = threadIdx.x; there && p0 < packs; p0 += ROW_THREADS * NARROW) {
+            Pack<T, N> g[NARROW], r[NARROW];
+            #pragma unroll
+            for (int u = 0; u < NARROW; ++u) {
+                if (p0 + u * ROW_THREADS >= packs) continue;
+                g[u].load(gradient + (p0 + u * ROW_THREADS) * N);
+                if (d_weights && counts) r[u].load(rows + row + (p0 + u * ROW_THREADS) * N);
+            }
+            #pragma unroll
+            for (int u = 0; u < NARROW; ++u) {
+                if (p0 + u * ROW_THREADS >= packs) continue;
+                float v[N];
+                #pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (d_weights && counts) dot = __fmaf_rn(g[u][i], r[u][i], dot);
+                    v[i] = w * g[u][i];
+                }
+                if (!d_rows) continue;
+                Pack<T, N> out;
+                out.set(v);
+                if (!counts) out.clear();
+                out.store(d_rows + row + (p0 + u * ROW_THREADS) * N);
+            }
+        }
+        if (!d_weights) continue;
+        __syncwarp();
+        #pragma unroll
+        for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, d);
+        if (threadIdx.x % 32 == 0) partial[j % 2][threadIdx.x / 32] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float sum = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < WARPS; ++i) sum += partial[j % 2][i];
+            d_weights[size_t(token) * topk + j] = sum;
+        }
+    }
+}
+
 void check_routes(int tokens, int topk, int hidden) {
     if (tokens < 0 || topk < 1 || hidden < 1) throw std::invalid_argument("tokens: topk and hidden must be positive, tokens not negative");
     if ((long long)(tokens) * topk > 0x7FFFFFFFll) throw std::invalid_argument("tokens: tokens * topk must be below 2^31");
 }
 
-bool whole_packs(int hidden, size_t size, std::initializer_list<const void*> pointers) {
-    uintptr_t bits = 0;
+// Values that can be moved at once: the largest power of two that divides a row and whose bytes divide the addresses.
+int pack_values(int hidden, size_t size, std::initializer_list<const void*> pointers) {
+    uintptr_t bits = uintptr_t(hidden) * size;
     for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
-    return size_t(hidden) * size % 16 == 0 && (bits & 15) == 0;
+    size_t bytes = 16;
+    while (bytes > size && (bits & (bytes - 1))) bytes /= 2;
+    return int(bytes / size);
 }
 
 // The grid of (token, segment of `per` packs) blocks.
@@ -337,11 +507,16 @@ unsigned blocks(int tokens, int packs, int per, int& segments) {
 
 // body(value of the type, number of values per pack)
 template <typename F>
-void by_type(int dtype, bool whole, F&& body) {
+void by_type(int dtype, int hidden, std::initializer_list<const void*> pointers, F&& body) {
     auto with = [&](auto value) {
         using T = decltype(value);
-        if (whole) body(value, std::integral_constant<int, int(16 / sizeof(T))>{});
-        else body(value, std::integral_constant<int, 1>{});
+        const int n = pack_values(hidden, sizeof(T), pointers);
+        if constexpr (sizeof(T) == 2) {
+            if (n == 8) return body(value, std::integral_constant<int, 8>{});
+        }
+        if (n == 4) return body(value, std::integral_constant<int, 4>{});
+        if (n == 2) return body(value, std::integral_constant<int, 2>{});
+        return body(value, std::integral_constant<int, 1>{});
     };
     switch (dtype) {
         case DTYPE_BF16: return with(__nv_bfloat16{});
@@ -350,44 +525,52 @@ void by_type(int dtype, bool whole, F&& body) {
         default: throw std::invalid_argument("tokens: dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)");
     }
 }
+// body(number of routes whose rows are in flight at once)
+template <typename F>
+void by_group(int topk, F&& body) {
+    if (topk <= 2) return body(std::integral_constant<int, 2>{});
+    if (topk <= 4) return body(std::integral_constant<int, 4>{});
+    if (topk <= 6) return body(std::integral_constant<int, 6>{});
+    return body(std::integral_constant<int, 8>{});
+}
 
-template <typename Id, int THREADS>
-void launch_sort(const void* ids, int routes, int experts, int* offsets, int* position, int* source, unsigned ctas, cudaStream_t stream) {
-    auto kernel = tokens_sort_kernel<Id, THREADS>;
-    const size_t smem = size_t(THREADS / 32 + 2) * (experts + 1) * sizeof(int);
-    if (smem > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    cudaLaunchAttribute attrs[2]{};
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim = {ctas, 1, 1};
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attrs;
-    cfg.numAttrs = 2;
-    cuda_check(cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), routes, experts, offsets, position, source));
+template <typename Id>
+void launch_sort(const Id* ids, int routes, int experts, int* offsets, int* position, int* source, int* counts, cudaStream_t stream) {
+    const size_t keys = size_t(experts) + 1;
     g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (routes <= SMALL) {
+        launch_chained(tokens_sort_small_kernel<Id>, dim3(1), dim3(SMALL), 0, stream, ids, routes, experts, offsets, position, source);
+        return;
+    }
+    int part;
+    const int blocks = sort_blocks(routes, part);
+    if (blocks > 1) {
+        launch_chained(tokens_count_kernel<Id>, dim3(unsigned(blocks)), dim3(BLOCK), keys * sizeof(int), stream, ids, routes, experts, part, counts);
+        g_launches.fetch_add(1, std::memory_order_relaxed);
+    }
+    const size_t smem = (SORT_WARPS + 2) * keys * sizeof(int);
+    if (smem > 48 * 1024) cuda_check(cudaFuncSetAttribute(tokens_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    launch_chained(tokens_sort_kernel<Id>, dim3(unsigned(blocks)), dim3(BLOCK), smem, stream, ids, routes, experts, part,
+                   blocks > 1 ? counts : nullptr, offsets, position, source);
 }
 
 }  // namespace
 
-void tokens_sort(const void* ids, int id_bytes, int routes, int experts, int* offsets, int* position, int* source, cudaStream_t stream) {
+size_t tokens_sort_workspace(int routes, int experts) {
+    int part;
+    const int blocks = routes > SMALL ? sort_blocks(routes, part) : 1;
+    return blocks > 1 ? size_t(blocks) * (size_t(experts) + 1) * sizeof(int) : 0;
+}
+
+void tokens_sort(const void* ids, int id_bytes, int routes, int experts, int* offsets, int* position, int* source, int* workspace,
+                 cudaStream_t stream) {
     if (experts < 1 || experts > SORT_MAX_EXPERTS) throw std::invalid_argument("tokens sort: 1..1024 experts");
     if (routes < 0) throw std::invalid_argument("tokens sort: the number of routes must not be negative");
     if (id_bytes != 4 && id_bytes != 8) throw std::invalid_argument("tokens sort: ids are 32- or 64-bit integers");
     if (!offsets || (routes > 0 && (!ids || !position || !source))) throw std::invalid_argument("tokens sort: null pointer");
-    // A small batch is sorted by one CTA of eight warps; from 2048 routes on eight CTAs of 32 share them.
-    const bool small = routes < 2048;
-    if (id_bytes == 8) {
-        if (small) launch_sort<long long, 256>(ids, routes, experts, offsets, position, source, 1, stream);
-        else launch_sort<long long, 1024>(ids, routes, experts, offsets, position, source, 8, stream);
-    } else {
-        if (small) launch_sort<int, 256>(ids, routes, experts, offsets, position, source, 1, stream);
-        else launch_sort<int, 1024>(ids, routes, experts, offsets, position, source, 8, stream);
-    }
+    if (!workspace && tokens_sort_workspace(routes, experts)) throw std::invalid_argument("tokens sort: a batch of this size needs its workspace");
+    if (id_bytes == 8) launch_sort(static_cast<const long long*>(ids), routes, experts, offsets, position, source, workspace, stream);
+    else launch_sort(static_cast<const int*>(ids), routes, experts, offsets, position, source, workspace, stream);
 }
 
 void tokens_gather(const void* x, int dtype, int tokens, int topk, int hidden, const int* position, const int* live, void* rows,
@@ -395,11 +578,11 @@ void tokens_gather(const void* x, int dtype, int tokens, int topk, int hidden, c
     check_routes(tokens, topk, hidden);
     if (tokens == 0) return;
     if (!x || !position || !live || !rows) throw std::invalid_argument("tokens gather: null pointer");
-    by_type(dtype, whole_packs(hidden, dtype_bytes(dtype), {x, rows}), [&](auto value, auto n) {
+    by_type(dtype, hidden, {x, rows}, [&](auto value, auto n) {
         using T = decltype(value);
         constexpr int N = decltype(n)::value;
         int segments;
-        const unsigned grid = blocks(tokens, hidden / N, ROW_THREADS * GATHER_PACKS, segments);
+        const unsigned grid = blocks(tokens, hidden / N, ROW_THREADS * GATHER_PACKS<T, N>, segments);
         launch_chained(tokens_gather_kernel<T, N>, dim3(grid), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(x),
                        static_cast<T*>(rows), position, live, tokens, topk, hidden, segments);
     });
@@ -411,14 +594,17 @@ void tokens_combine(const void* rows, int dtype, const float* weights, const int
     check_routes(tokens, topk, hidden);
     if (tokens == 0) return;
     if (!rows || !position || !live || !y) throw std::invalid_argument("tokens combine: null pointer");
-    by_type(dtype, whole_packs(hidden, dtype_bytes(dtype), {rows, y}), [&](auto value, auto n) {
+    by_type(dtype, hidden, {rows, y}, [&](auto value, auto n) {
         using T = decltype(value);
         constexpr int N = decltype(n)::value;
         int segments;
-        const unsigned grid = blocks(tokens, hidden / N, ROW_THREADS, segments);
-        auto kernel = weights ? tokens_combine_kernel<T, N, true> : tokens_combine_kernel<T, N, false>;
-        launch_chained(kernel, dim3(grid), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(rows), weights, position, live, tokens,
-                       topk, hidden, segments, static_cast<T*>(y));
+        const unsigned grid = blocks(tokens, hidden / N, sizeof(T) * N == 16 ? ROW_THREADS : ROW_THREADS * NARROW, segments);
+        auto go = [&](auto kernel) {
+            launch_chained(kernel, dim3(grid), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(rows), weights, position, live,
+                           tokens, topk, hidden, segments, static_cast<T*>(y));
+        };
+        if constexpr (sizeof(T) * N == 16) by_group(topk, [&](auto group) { go(tokens_combine_kernel<T, decltype(group)::value>); });
+        else go(tokens_combine_narrow_kernel<T, N>);
     });
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
@@ -428,11 +614,15 @@ void tokens_combine_backward(const void* d_y, int dtype, const void* rows, const
     check_routes(tokens, topk, hidden);
     if (tokens == 0 || (!d_rows && !d_weights)) return;
     if (!d_y || !weights || !position || !live || (d_weights && !rows)) throw std::invalid_argument("tokens combine backward: null pointer");
-    by_type(dtype, whole_packs(hidden, dtype_bytes(dtype), {d_y, rows, d_rows}), [&](auto value, auto n) {
+    by_type(dtype, hidden, {d_y, rows, d_rows}, [&](auto value, auto n) {
         using T = decltype(value);
         constexpr int N = decltype(n)::value;
-        launch_chained(tokens_combine_backward_kernel<T, N>, dim3(unsigned(tokens)), dim3(256), 0, stream, static_cast<const T*>(d_y),
-                       static_cast<const T*>(rows), weights, position, live, tokens, topk, hidden, static_cast<T*>(d_rows), d_weights);
+        auto go = [&](auto kernel) {
+            launch_chained(kernel, dim3(unsigned(tokens)), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(d_y),
+                           static_cast<const T*>(rows), weights, position, live, tokens, topk, hidden, static_cast<T*>(d_rows), d_weights);
+        };
+        if constexpr (sizeof(T) * N == 16) by_group(topk, [&](auto group) { go(tokens_combine_backward_kernel<T, decltype(group)::value>); });
+        else go(tokens_combine_backward_narrow_kernel<T, N>);
     });
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }

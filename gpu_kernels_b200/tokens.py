@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .int8 import aligned
+from .int8 import aligned, matrix
 from .nvfp4 import _DTYPES, _require_cuda
 
 
@@ -42,13 +42,16 @@ def sort_routes(ids: torch.Tensor, num_experts: int) -> Routes:
     routes, d = ids.numel(), ids.device
     if routes >= 1 << 31:
         raise ValueError("fewer than 2^31 routes")
-    offsets = torch.empty((num_experts + 1,), dtype=torch.int32, device=d)
-    position = torch.empty(ids.shape, dtype=torch.int32, device=d)
-    source = torch.empty((routes,), dtype=torch.int32, device=d)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=d)
+    position = matrix(*ids.shape, torch.int32, d)
+    source = torch.empty(routes, dtype=torch.int32, device=d)
+    lib = _lib.load()
+    needed = lib.gpu_kernels_tokens_sort_workspace(routes, num_experts)
+    room = torch.empty(needed, dtype=torch.uint8, device=d) if needed else None
     with _lib.on(d):
-        _lib.check(_lib.load().gpu_kernels_tokens_sort(
+        _lib.check(lib.gpu_kernels_tokens_sort(
             ids.data_ptr(), ids.element_size(), routes, num_experts, offsets.data_ptr(), position.data_ptr(), source.data_ptr(),
-            _lib.stream()))
+            None if room is None else room.data_ptr(), _lib.stream()))
     return Routes(offsets, position, source)
 
 
@@ -75,7 +78,7 @@ def _values(t: torch.Tensor, name: str) -> torch.Tensor:
 def _gather(x, routes):
     x = x.contiguous()
     position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
-    rows = torch.empty((tokens * topk, x.shape[1]), dtype=x.dtype, device=x.device)
+    rows = matrix(tokens * topk, x.shape[1], x.dtype, x.device)
     with _lib.on(x.device):
         _lib.check(_lib.load().gpu_kernels_tokens_gather(
             x.data_ptr(), _DTYPES[x.dtype], tokens, topk, x.shape[1], position, live, rows.data_ptr(), _lib.stream()))
@@ -85,7 +88,7 @@ def _gather(x, routes):
 def _combine(rows, routes, weights):
     rows = rows.contiguous()
     position, live, tokens, topk = _check_routes(routes, None, rows.device)
-    y = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    y = matrix(tokens, rows.shape[1], rows.dtype, rows.device)
     with _lib.on(rows.device):
         _lib.check(_lib.load().gpu_kernels_tokens_combine(
             rows.data_ptr(), _DTYPES[rows.dtype], None if weights is None else weights.data_ptr(), position, live, tokens, topk,
@@ -122,9 +125,9 @@ class _CombineTokens(torch.autograd.Function):
         position, live, tokens, topk = _check_routes(routes, d_y.shape[0], d_y.device)
         d_rows = d_weights = None
         if ctx.needs_input_grad[0]:
-            d_rows = torch.empty((tokens * topk, d_y.shape[1]), dtype=d_y.dtype, device=d_y.device)
+            d_rows = matrix(tokens * topk, d_y.shape[1], d_y.dtype, d_y.device)
         if ctx.needs_input_grad[1]:
-            d_weights = torch.empty((tokens, topk), dtype=torch.float32, device=d_y.device)
+            d_weights = matrix(tokens, topk, torch.float32, d_y.device)
             rows = rows.contiguous()
         with _lib.on(d_y.device):
             _lib.check(_lib.load().gpu_kernels_tokens_combine_backward(
@@ -147,13 +150,13 @@ def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
 def gather_tokens_int8(x: torch.Tensor, routes: Routes):
     """quantize_int8(x) in the order of the routes: x [T, K] -> (codes int8 [T * topk, K], scales fp32 [T * topk]), the rows
     `int8_grouped_gemm` takes. A token is quantised once, K a multiple of 16; rows of no expert have codes and scale 0."""
-    x = aligned(_values(x, "x").detach())
+    x = aligned(_values(x, "x"))
     position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
     k = x.shape[1]
     if k % 16:
         raise ValueError("K must be a multiple of 16")
-    codes = torch.empty((tokens * topk, k), dtype=torch.int8, device=x.device)
-    scales = torch.empty((tokens * topk,), dtype=torch.float32, device=x.device)
+    codes = matrix(tokens * topk, k, torch.int8, x.device)
+    scales = torch.empty(tokens * topk, dtype=torch.float32, device=x.device)
     with _lib.on(x.device):
         _lib.check(_lib.load().gpu_kernels_tokens_gather_int8(
             x.data_ptr(), _DTYPES[x.dtype], tokens, topk, k, position, live, codes.data_ptr(), scales.data_ptr(), _lib.stream()))

@@ -49,9 +49,11 @@ int gpu_kernels_int8_tiles(int rows, int N, int K, int experts, int* info);
 /* ids [routes] int32 or int64 (id_bytes 4 or 8): offsets [experts + 1], position [routes] = row of each route,
  * source [routes] = route of each row, int32 each. Rows are ordered by expert, then by route; routes of no expert (ids
  * outside [0, experts)) come last, from row offsets[experts] on. At most 1024 experts. 4-byte aligned pointers (ids: 8
- * where 64-bit). */
+ * where 64-bit). workspace: gpu_kernels_tokens_sort_workspace bytes of the caller's (NULL where that is 0), not shared
+ * with a call that may run at the same time. */
 int gpu_kernels_tokens_sort(const void* ids, int id_bytes, int routes, int experts, void* offsets, void* position, void* source,
-                            void* stream);
+                            void* workspace, void* stream);
+size_t gpu_kernels_tokens_sort_workspace(int routes, int experts);
 /* rows [tokens * topk, hidden]: x [tokens, hidden] in that order; `live` points to the number of live rows
  * (offsets + experts); the rows behind are cleared. A position outside the rows is skipped. Pointers need the alignment of
  * their type only; 16-byte aligned rows are copied 16 bytes at a time. */

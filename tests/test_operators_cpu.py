@@ -17,7 +17,7 @@ def test_symbols_are_exported_and_bound():
     from gpu_kernels_b200 import _lib, build
     lib = ctypes.CDLL(str(build.build()))
     names = declared_symbols()
-    assert len(names) == 11 and sorted(_lib.OPERATOR_SIGNATURES) == names
+    assert len(names) == 12 and sorted(_lib.OPERATOR_SIGNATURES) == names
     for name in names:
         assert hasattr(lib, name), name
 
@@ -29,7 +29,7 @@ def test_fails_loudly_without_gpu():
     with pytest.raises(_lib.Nvfp4Error):
         _lib.check(_lib.load().gpu_kernels_int8_quantize(None, 0, None, None, 1, 16, None))
     with pytest.raises(_lib.Nvfp4Error):
-        _lib.check(_lib.load().gpu_kernels_tokens_sort(None, 8, 0, 4, None, None, None, None))
+        _lib.check(_lib.load().gpu_kernels_tokens_sort(None, 8, 0, 4, None, None, None, None, None))
 
 
 def test_cpu_tensors_are_refused():

@@ -42,7 +42,8 @@ def check_order(g, ids, experts):
 
 
 @pytest.mark.parametrize("tokens,topk,experts", ((1, 1, 1), (1, 6, 256), (5, 3, 2), (32, 1, 7), (31, 2, 1024), (333, 6, 255),
-                                                 (255, 8, 64), (256, 8, 64), (1000, 4, 1024), (2731, 6, 33), (20000, 3, 257)))
+                                                 (32, 8, 64), (255, 8, 64), (256, 4, 64),
+                                                 (1025, 1, 3), (256, 8, 64), (1000, 4, 1024), (2731, 6, 33), (20000, 3, 257), (80000, 2, 100)))
 def test_order(g, tokens, topk, experts):
     check_order(g, choices(tokens, topk, experts, tokens, 0.1), experts)
     check_order(g, choices(tokens, topk, experts, tokens + 5).int(), experts)
@@ -74,7 +75,7 @@ def live_routes(routes):
     return routes.position < routes.offsets[-1]
 
 
-SHAPES = ((1, 1, 1, 1), (1, 6, 256, 4096), (7, 3, 4, 33), (20, 2, 5, 64), (64, 6, 16, 1000), (33, 9, 40, 257), (5, 17, 20, 2056), (300, 8, 64, 512))
+SHAPES = ((1, 1, 1, 1), (9, 4, 8, 1030), (6, 2, 8, 12), (11, 5, 8, 66), (1, 6, 256, 4096), (7, 3, 4, 33), (20, 2, 5, 64), (64, 6, 16, 1000), (33, 9, 40, 257), (5, 17, 20, 2056), (300, 8, 64, 512))
 
 
 @pytest.mark.parametrize("dtype", (BF16, F16, F32))
