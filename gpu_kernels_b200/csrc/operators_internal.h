@@ -30,6 +30,7 @@ struct Int8Tiles {
     int width;      // values of the MMA's N side per tile
     int split;      // CTAs that share a tile's K loop (one cluster)
     int stages;
+    int subs;       // boxes of 128 K values per operand and ring stage
 };
 // rows x n x k; experts > 0: rows dealt to that many experts.
 Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device);

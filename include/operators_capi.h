@@ -26,7 +26,7 @@ int gpu_kernels_int8_quantize(const void* x, int dtype, void* codes, void* scale
 /* codes * scale -> fp32 [rows, K]. */
 int gpu_kernels_int8_dequantize(const void* codes, const void* scales, void* out_f32, long long rows, int K, void* stream);
 /* C [M, N] = (a [M, K] b [N, K]^T) * a_scales[m] * b_scales[n]: exact integer sums, FP32 scaling, rounded to C's type.
- * K a multiple of 16, at most 131056; N a multiple of 8; any M. a_scales 4-byte aligned. Any int8 code, -128 included. */
+ * K a multiple of 16, at most 131056; N a multiple of 8; M and N up to 2^30. a_scales 4-byte aligned. Any int8 code, -128 included. */
 int gpu_kernels_int8_gemm(const void* a, const void* b, const void* a_scales, const void* b_scales, void* C, int out_dtype,
                           int M, int N, int K, void* stream);
 /* The same for activations x [M, K] that are quantised on the way; codes [M, K] and scales [M] are workspace and hold what
@@ -36,7 +36,7 @@ int gpu_kernels_int8_linear(const void* x, int dtype, const void* b, const void*
 /* rows [R, K] sorted by expert, offsets [experts + 1] int32 (device): expert e's rows are [offsets[e], offsets[e + 1]) and
  * are multiplied by weights[e] of [experts, N, K] (scales [experts, N]); C [R, N]. Rows of no expert (in front of
  * offsets[0], at or behind offsets[experts]) are left as they were, or with zero_rest cleared. At most 1024 experts,
- * experts * N below 2^31. Offsets are clipped to 0..R; where they decrease, the largest so far counts. */
+ * experts * N up to 2^30. Offsets are clipped to 0..R; where they decrease, the largest so far counts. */
 int gpu_kernels_int8_grouped_gemm(const void* rows, const void* weights, const void* row_scales, const void* weight_scales,
                                   const void* offsets, int experts, void* C, int out_dtype, int R, int N, int K, int zero_rest,
                                   void* stream);

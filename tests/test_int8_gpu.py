@@ -138,7 +138,8 @@ def assert_product(c, want):
 
 SIZES = ((1, 8, 16), (1, 128, 128), (2, 136, 4096), (7, 264, 144), (16, 1024, 4096), (17, 512, 2064), (64, 200, 2048),
          (96, 2048, 8192), (128, 1000, 512), (130, 384, 272), (200, 136, 1040), (256, 512, 1024), (257, 520, 400),
-         (300, 1000, 992), (513, 2056, 640), (700, 264, 3184), (1024, 1024, 1024))
+         (300, 1000, 992), (513, 2056, 640), (700, 264, 3184), (1024, 1024, 1024),
+         (9, 8192, 4096), (5, 18944, 1024), (128, 28672, 272), (300, 8200, 528))
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -156,9 +157,9 @@ def test_product(g, m, n, k):
 
 def test_every_kernel_is_reached(g):
     tiles = [g.int8_tiles(*size) for size in SIZES]
-    assert {t["pair"] for t in tiles} == {0, 1}
-    assert {t["split"] for t in tiles} >= {1, 2, 4, 8}
-    assert {t["width"] for t in tiles if t["swap"]} >= {16, 32, 64, 96, 128}
+    assert {(t["pair"], t["swap"]) for t in tiles} == {(1, 0), (0, 0), (0, 1)}
+    assert {t["split"] for t in tiles if t["swap"]} == {1, 2, 4, 8}
+    assert {t["width"] for t in tiles if t["swap"]} >= {16, 32, 96} and {t["width"] for t in tiles if t["pair"]} >= {32, 64, 96}
 
 
 @pytest.mark.parametrize("m", (1, 300))
