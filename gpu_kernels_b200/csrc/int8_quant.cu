@@ -7,7 +7,8 @@
 //
 // HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes. Threads take 16
 // values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
-// and stores are aligned whatever K is; a row that starts or ends inside a group takes that group value by value.
+// and stores are aligned whatever K is; what a row has in front of its first whole group and behind its last one (up to 15
+// values each) is taken by 32 threads, one value each.
 #include "operators_internal.h"
 #include "ptx.cuh"
 
@@ -83,23 +84,6 @@ struct Group {                                                  // 16 values as 
         #pragma unroll
         for (int i = 0; i < int(sizeof(T)); ++i) raw[i] = __ldg(p + i);
     }
-    // Only the elements [begin, end) of the flat array; zeros for the others, which raise no maximum.
-    __device__ __forceinline__ void load_part(const T* x, size_t group, size_t begin, size_t end) {
-        using U = typename std::conditional<sizeof(T) == 2, unsigned short, uint32_t>::type;
-        const U* p = reinterpret_cast<const U*>(x);
-        uint32_t w[4 * sizeof(T)];
-        #pragma unroll
-        for (int i = 0; i < int(4 * sizeof(T)); ++i) w[i] = 0u;
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const size_t at = group * 16 + i;
-            const uint32_t v = at >= begin && at < end ? uint32_t(__ldg(p + at)) : 0u;
-            if constexpr (sizeof(T) == 2) w[i / 2] |= v << (16 * (i % 2));
-            else w[i] = v;
-        }
-        #pragma unroll
-        for (int i = 0; i < int(sizeof(T)); ++i) raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    }
     __device__ __forceinline__ uint32_t magnitude(uint32_t sofar) const {   // 16-bit types: two maxima side by side
         #pragma unroll
         for (int i = 0; i < int(4 * sizeof(T)); ++i) {
@@ -127,9 +111,9 @@ struct Group {                                                  // 16 values as 
     }
 };
 
-// TPR: threads per row, NV: groups of 16 that each of them holds in registers (0: any number, the row is read twice, the
-// second time from L2). ROUTED: the row's codes go to `topk` rows of the output instead of its own.
-template <typename T, int TPR, int NV, bool ROUTED>
+// TPR: threads per row, NV: groups of 16 that each of them holds in registers; what a row has beyond TPR * NV groups is read
+// twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
+template <typename T, int TPR, int NV, bool ROUTED, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, long long rows, int K,
                      const int* __restrict__ position, const int* __restrict__ live, int topk) {
@@ -139,26 +123,29 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
     const long long row = (long long)(blockIdx.x) * ROWS + threadIdx.x / TPR;
     if (TPR == 32 && row >= rows) return;                       // (a warp's row; otherwise the grid has one block per row)
     const size_t begin = size_t(row) * K, end = begin + K;
-    const size_t g0 = begin / 16, g1 = (end + 15) / 16;
-    auto fetch = [&](Group<T>& v, size_t group) {
-        if (group * 16 >= begin && group * 16 + 16 <= end) v.load(x, group);
-        else v.load_part(x, group, begin, end);
-    };
-    Group<T> held[NV > 0 ? NV : 1];
-    uint32_t top = 0u;
-    if constexpr (NV > 0) {
-        #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (g0 + t + j * TPR < g1) fetch(held[j], g0 + t + j * TPR);
-        #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (g0 + t + j * TPR < g1) top = held[j].magnitude(top);
-    } else {
-        for (size_t group = g0 + t; group < g1; group += TPR) {
-            fetch(held[0], group);
-            top = held[0].magnitude(top);
-        }
+    const size_t whole_from = WHOLE ? begin : min(end, (begin + 15) / 16 * 16), whole_to = WHOLE ? end : max(whole_from, end / 16 * 16);
+    const size_t g0 = whole_from / 16, g1 = g0 + (whole_to - whole_from) / 16;
+    // This thread's value outside the whole groups: in front of them for the first sixteen threads, behind for the next.
+    const size_t single = t < 16 ? begin + t : whole_to + (t - 16);
+    const bool has_single = !WHOLE && t < 32 && single < (t < 16 ? whole_from : end);
+    uint32_t single_bits = 0u;
+    if (has_single) {
+        if constexpr (sizeof(T) == 2) single_bits = __ldg(reinterpret_cast<const unsigned short*>(x) + single);
+        else single_bits = __ldg(reinterpret_cast<const uint32_t*>(x) + single);
     }
+    Group<T> held[NV];
+    uint32_t top = single_bits & (sizeof(T) == 2 ? 0x7FFFu : 0x7FFFFFFFu);
+    #pragma unroll
+    for (int j = 0; j < NV; ++j)
+        if (g0 + t + j * TPR < g1) held[j].load(x, g0 + t + j * TPR);
+    for (size_t group = g0 + t + NV * TPR; !WHOLE && group < g1; group += TPR) {
+        Group<T> v;
+        v.load(x, group);
+        top = v.magnitude(top);
+    }
+    #pragma unroll
+    for (int j = 0; j < NV; ++j)
+        if (g0 + t + j * TPR < g1) top = held[j].magnitude(top);
     if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     if constexpr (TPR > 32) {
@@ -181,24 +168,18 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
                 if (to < 0 || to >= out_rows) continue;
                 reinterpret_cast<uint4*>(codes)[size_t(to) * (K / 16) + (group - g0)] = to < end_live ? c : make_uint4(0u, 0u, 0u, 0u);
             }
-        } else if (group * 16 >= begin && group * 16 + 16 <= end) {
-            reinterpret_cast<uint4*>(codes)[group] = c;
         } else {
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (group * 16 + i >= begin && group * 16 + i < end) codes[group * 16 + i] = int8_t(w[i / 4] >> (8 * (i % 4)));
+            reinterpret_cast<uint4*>(codes)[group] = c;
         }
     };
-    if constexpr (NV > 0) {
-        #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (g0 + t + j * TPR < g1) emit(held[j], g0 + t + j * TPR);
-    } else {
-        for (size_t group = g0 + t; group < g1; group += TPR) {
-            fetch(held[0], group);
-            emit(held[0], group);
-        }
+    if (has_single) codes[single] = finite ? int8_t(code_of<T>(Bits<T>::widen(single_bits), s)) : int8_t(0);
+    #pragma unroll
+    for (int j = 0; j < NV; ++j)
+        if (g0 + t + j * TPR < g1) emit(held[j], g0 + t + j * TPR);
+    for (size_t group = g0 + t + NV * TPR; !WHOLE && group < g1; group += TPR) {
+        Group<T> v;
+        v.load(x, group);
+        emit(v, group);
     }
     if constexpr (ROUTED) {
         const int end_live = __ldg(live);
@@ -251,14 +232,23 @@ void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, 
         launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads), 0, stream,
                        static_cast<const T*>(x), codes, scales, rows, K, position, live, topk);
     };
-    const int groups = K % 16 == 0 ? K / 16 : K / 16 + 2;       // a row that starts inside a group reaches one more
-    if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED>, 256, 8);
-    else if (groups <= 128) go(int8_quantise_kernel<T, 32, 4, ROUTED>, 256, 8);
-    else if (groups <= 256) go(int8_quantise_kernel<T, 256, 1, ROUTED>, 256, 1);
-    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED>, 256, 1);
-    else if (groups <= 1024) go(int8_quantise_kernel<T, 256, 4, ROUTED>, 256, 1);
-    else if (groups <= 2048) go(int8_quantise_kernel<T, 512, 4, ROUTED>, 512, 1);
-    else go(int8_quantise_kernel<T, 512, 0, ROUTED>, 512, 1);
+    const int groups = K / 16;
+    // A group held is 8 registers of 16-bit values and 16 of FP32: of those no more than two (four left room for two blocks
+    // per SM: 4096 x 16384 FP32 71 us, 8192 x 1024 14 us), but for the longest rows.
+    constexpr bool SHORT = sizeof(T) == 2;
+    constexpr int MOST = SHORT ? 4 : 2;
+    if (K % 16 || groups > 2048) {
+        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
+        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, 256, 1);
+        else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, 512, 1);
+    } else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 256, 8);
+    else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 256, 8);
+    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 256, 8);
+    else if (groups <= 256) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, 256, 1);
+    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, 256, 1);
+    else if (groups <= 256 * MOST) go(int8_quantise_kernel<T, 256, MOST, ROUTED, true>, 256, 1);
+    else if (groups <= 1024) go(int8_quantise_kernel<T, 512, 2, ROUTED, true>, 512, 1);
+    else go(int8_quantise_kernel<T, 512, 4, ROUTED, true>, 512, 1);
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
