@@ -473,10 +473,12 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         ctrl->wait.abort = 0;
         mbar_init_fence();
     }
-    if (warp == 4) {
-        tmem_alloc<CG>(smem_u32(&ctrl->tmem_base), columns);
-        tmem_relinquish<CG>();
-    }
+    // A pair allocates Tensor Memory together: both CTAs have to be there before either begins, and stay until both have
+    // given it back. (Without this barrier a CTA that was launched later than its partner, its SM still busy with the
+    // kernel in front, never got out of its allocation.)
+    __syncwarp();
+    if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); }
+    if (warp == 4) tmem_alloc<CG>(smem_u32(&ctrl->tmem_base), columns);
     if (warp == 5 && lane == 0) { prefetch_tensormap(&mapX); prefetch_tensormap(&mapY); }
     if (!g.early) chain_point();
     if (g.offsets) {
@@ -515,10 +517,12 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         }
         __syncwarp();
     }
+    __syncwarp();
     tc_fence_before_sync();
     if (cluster) { cluster_arrive(); cluster_wait(); }
     __syncthreads();
     tc_fence_after_sync();
+    if (warp == 4) tmem_relinquish<CG>();
     const uint32_t tmem = ctrl->tmem_base;
 
     const int members = CG == 2 ? 2 : g.split;
@@ -557,7 +561,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     if (warp == 4) {
         tc_fence_after_sync();
         tmem_dealloc<CG>(tmem, columns);
+        __syncwarp();
     }
+    if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
