@@ -1005,9 +1005,13 @@ nvfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         ctrl->wait.abort = 0;
         mbar_init_fence();
     }
+    // A pair allocates Tensor Memory together: both CTAs have to be there before either begins, and stay until both have
+    // given it back. A CTA that is launched later than its partner (its SM still busy with the kernel in front, which
+    // programmatic launch allows) may otherwise never get out of its allocation.
+    if constexpr (CG == 2) { __syncwarp(); cluster_arrive(); cluster_wait(); }
     if (warp == 4) {
         tmem_alloc<CG>(smem_u32(&ctrl->tmem_base), TMEM_COLS);
-        tmem_relinquish<CG>();
+        if constexpr (CG == 1) tmem_relinquish<CG>();
     }
     if (warp == 5 && lane == 0) {
         prefetch_tensormap(&tmA); prefetch_tensormap(&tmB);
@@ -1021,9 +1025,11 @@ nvfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         asm volatile("mov.u32 %0, %%smid;" : "=r"(smid));
         if (smid < 256u && __ldg(g.sm_side + smid) != __ldg(g.unit_side + unit)) atomicAdd(g.status + 3, 1u);
     }
+    __syncwarp();
     tc_fence_before_sync();
     if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
     tc_fence_after_sync();
+    if (CG == 2 && warp == 4) tmem_relinquish<CG>();             // (for both CTAs of the pair)
     const uint32_t tmem = ctrl->tmem_base;
     // Everything above touched only this CTA's own resources. From here on global memory is read and written:
     // wait for the grid this launch depends on (returns at once when the launch was an ordinary one), unless the
@@ -1061,6 +1067,7 @@ nvfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         tc_fence_after_sync();
         tmem_dealloc<CG>(tmem, TMEM_COLS);
     }
+    if constexpr (CG == 2) { __syncwarp(); cluster_arrive(); cluster_wait(); }
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.cycles = uint32_t(clock64() - entered);
 }
 
