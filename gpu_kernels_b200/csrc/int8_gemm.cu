@@ -6,20 +6,23 @@
 // A warp-specialised kernel of 320 threads per CTA: warp 5 streams tiles of both operands through a ring in shared memory
 // by TMA (128 bytes of K per row and stage, 128-byte swizzle), warp 4 issues tcgen05.mma.kind::i8 from it, and warps 0-3
 // and 6-9, two per Tensor Memory lane quarter, drain the accumulators. Two accumulators take turns, so that a tile is
-// drained while the next one is computed. Three forms, all persistent but the split one:
+// drained while the next one is computed. The forms, all persistent but the split one:
 //   CTA pairs: 256 tokens on the MMA's M side, up to 256 channels on its N side. For many tokens: bound by the tensor cores.
 //   Single CTAs: the same with up to 128 tokens and as many channels to a tile (in steps of 16) as give each SM one tile.
 //   SWAP, single CTAs: 128 channels on the M side, the tokens on the N side, in as narrow a tile as holds them. For few
 //     tokens, where each weight byte is read once and HBM is the bound. Where the tiles are fewer than the SMs, a cluster of
 //     2, 4 or 8 CTAs shares a tile's K loop: their integer partial sums meet in distributed shared memory, and the order in
 //     which they are added does not matter.
+//   Grouped, SWAP, single CTAs or pairs (256 channels): rows sorted by expert, `offsets` (device) says where each expert's
+//     rows start, the weights are stacked [experts, N, K]. Every CTA counts the experts' tiles once and walks the same
+//     sequence, an expert's tokens innermost, so that its weights are read from HBM once. An expert's rows are dealt evenly
+//     to as few tiles as hold them; the MMA's N and the rows a tile fetches (32 to a box) follow its share. With tiles of
+//     one width for all, 256 experts of unequal popularity took 1143 us instead of 891 in a loop (4096 tokens of six
+//     routes). A tile that reaches into the next expert's rows (or channels) computes them with the wrong weights and does
+//     not store them.
 // Measured: 8192 cubed 331 us (3.32 POPS, twice the rate cuBLAS reaches in bf16); 1 x 8192 x 8192 15.2 us (4.4 TB/s), 1 x
 // 28672 x 8192 40.4 us (5.8 TB/s), 128 x 28672 x 8192 44 us; 256 experts of 4096 x 4096 with 64 tokens of six routes each
-// 470 us (7.1 TB/s), with 4096 tokens 690 us (6.7 TB/s; 842 where experts differ in popularity).
-// Grouped: rows sorted by expert, `offsets` (device) says where each expert's rows start, and the weights are stacked
-// [experts, N, K]. Every CTA counts the experts' tiles once and walks the same sequence, an expert's tokens innermost, so
-// that its weights are read from HBM once. A tile that reaches into the next expert's rows (or channels) computes them
-// with the wrong weights and does not store them.
+// 470 us (7.1 TB/s).
 #include "operators_internal.h"
 #include "ptx.cuh"
 
@@ -71,6 +74,7 @@ struct Args {
 
 struct Tile {
     int x, y;                       // first row in the M side's and in the N side's operand
+    int n;                          // values on the N side: g.width, or in a grouped product as few as hold the tile's tokens
     int token, token_end;           // first row of C, and the first one that is not this tile's to write
     int channel;                    // first column of C
     int scale;                      // first channel in b_scale
@@ -94,11 +98,13 @@ struct Walk {
         Tile r;
         if (g.offsets) {
             while (tile_start[expert + 1] <= t) ++expert;
-            const int row0 = row_start[2 * expert], row1 = row_start[2 * expert + 1], local = t - tile_start[expert];
-            const int per = SWAP ? g.width : X, count = (row1 - row0 + per - 1) / per;
-            const int channel_tile = local / count, token_tile = local - channel_tile * count;
+            const int row0 = row_start[2 * expert], row1 = row_start[2 * expert + 1], rows = row1 - row0, local = t - tile_start[expert];
+            int per = SWAP ? g.width : X;
+            const int count = (rows + per - 1) / per, channel_tile = local / count, token_tile = local - channel_tile * count;
+            if (SWAP) per = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);         // equal shares, no more than g.width
             r.token = row0 + token_tile * per;
-            r.token_end = row1;
+            r.token_end = min(row1, r.token + per);
+            r.n = SWAP ? (r.token_end - r.token + 16 * CG - 1) / (16 * CG) * (16 * CG) : g.width;
             r.channel = channel_tile * (SWAP ? X : g.width);
             r.scale = expert * g.N + r.channel;
         } else {
@@ -107,8 +113,9 @@ struct Walk {
             const int per_band = g.band * g.tiles_y, b = t / per_band, first = b * g.band;
             const int high = min(g.band, g.tiles_x - first), within = t - b * per_band, column = within / high;
             const int tx = first + within - column * high, ty = (b & 1) ? g.tiles_y - 1 - column : column;
+            r.n = g.width;
             r.token = SWAP ? ty * g.width : tx * X;
-            r.token_end = g.M;
+            r.token_end = SWAP ? min(g.M, r.token + g.width) : g.M;
             r.channel = SWAP ? tx * X : ty * g.width;
             r.scale = r.channel;
         }
@@ -188,43 +195,56 @@ struct Roles {
     }
 
     // ---- warp 5 ---------------------------------------------------------------------------------------------------
+    // A place in the sequence of ring steps, with what a tile's requests need, computed once per tile.
     struct Cursor {
         Walk<CG, SWAP> walk;
-        Tile tile;
-        int ks, k0, k1;
-        __device__ Cursor(const Walk<CG, SWAP>& w, int a, int b) : walk(w), ks(a), k0(a), k1(b) {
-            if (walk.valid()) tile = walk.tile();
-        }
+        int ks, k0, k1, rank;
+        int x, y;                   // first rows of this CTA's part (of a pair, its half) of both operands
+        int parts;                  // boxes the tile takes on the N side: one, in a grouped product as many as hold its tokens
+        uint32_t bytes;             // of all boxes of 128 K values, in both CTAs of a pair
+        __device__ Cursor(const Walk<CG, SWAP>& w, int a, int b, int r) : walk(w), ks(a), k0(a), k1(b), rank(r) { enter(); }
         __device__ bool valid() const { return walk.valid(); }
+        __device__ void enter() {
+            if (!walk.valid()) return;
+            const Args& g = walk.g;
+            const Tile t = walk.tile();
+            x = t.x + (CG == 2 ? rank * 128 : 0);
+            y = t.y + (CG == 2 ? rank * (t.n / 2) : 0);
+            parts = SWAP && g.offsets ? (t.n / CG + g.y_box - 1) / g.y_box : 1;
+            bytes = uint32_t(CG) * uint32_t(g.x_box + parts * g.y_box) * ROW_BYTES;
+        }
         __device__ void next() {
             if (++ks < k1) return;
             ks = k0;
             walk.next();
-            if (walk.valid()) tile = walk.tile();
+            enter();
         }
     };
     // Boxes of a ring step that lie in K: those beyond would be zeros.
     __device__ __forceinline__ int boxes(int ks) const { return SUBS<CG> == 1 ? 1 : min(g.subs, g.kboxes - ks * g.subs); }
     // One operand's part of ring stage `stage`; x_side: the M side's.
     __device__ __forceinline__ void request(const CUtensorMap* map, bool x_side, const Cursor& c, int stage) const {
+        constexpr int MOST = SWAP ? 4 : 1;                      // boxes of 32 rows in 128 (a pair: 256 / 2)
         const uint32_t dst = smem + stage * stage_bytes + (x_side ? 0u : uint32_t(g.subs) * 128u * ROW_BYTES);
-        const uint32_t full = smem_u32(&ctrl->full[stage]);
-        if constexpr (CG == 1) {
-            const uint32_t pitch = (x_side ? 128u : uint32_t(g.width)) * ROW_BYTES;
-            const int n = boxes(c.ks);
+        const uint32_t full = smem_u32(&ctrl->full[stage]), bar = CG == 2 ? map_to_cta(full, 0) : full;
+        const uint32_t pitch = (x_side ? 128u : uint32_t(g.width / CG)) * ROW_BYTES, part = uint32_t(g.y_box) * ROW_BYTES;
+        const int n = boxes(c.ks);
+        #pragma unroll
+        for (int s = 0; s < SUBS<CG>; ++s) {
+            if (s >= n) break;
+            const int k = (c.ks * g.subs + s) * ROW_BYTES;
             #pragma unroll
-            for (int s = 0; s < SUBS<CG>; ++s)
-                if (s < n) tma_load_2d(dst + s * pitch, map, (c.ks * g.subs + s) * ROW_BYTES, x_side ? c.tile.x : c.tile.y, full);
-        } else {
-            const int half = x_side ? 128 : g.width / 2;        // each CTA of the pair loads its half of both operands
-            tma_load_2d_pair(dst, map, c.ks * ROW_BYTES, (x_side ? c.tile.x : c.tile.y) + int(rank) * half, map_to_cta(full, 0));
+            for (int p = 0; p < (x_side ? 1 : MOST); ++p) {
+                if (p >= (x_side ? 1 : c.parts)) break;
+                if constexpr (CG == 1) tma_load_2d(dst + s * pitch + p * part, map, k, (x_side ? c.x : c.y) + p * g.y_box, bar);
+                else tma_load_2d_pair(dst + s * pitch + p * part, map, k, (x_side ? c.x : c.y) + p * g.y_box, bar);
+            }
         }
     }
     __device__ void produce(const CUtensorMap* mapX, const CUtensorMap* mapY, int lane) const {
-        const uint32_t bytes = uint32_t(CG) * uint32_t(g.x_box + g.y_box) * ROW_BYTES;
         const CUtensorMap* weights = SWAP ? mapX : mapY;
         const CUtensorMap* tokens = SWAP ? mapY : mapX;
-        Cursor cursor(Walk<CG, SWAP>(g, tile_start, row_start, unit, units), k0, k1);
+        Cursor cursor(Walk<CG, SWAP>(g, tile_start, row_start, unit, units), k0, k1, int(rank));
         int stage = 0;
         uint32_t phase = 0;
         if (g.early) {
@@ -233,7 +253,7 @@ struct Roles {
             int lead = 0;
             for (; lead < g.stages && ahead.valid(); ++lead, ahead.next())
                 if (elect_one()) {
-                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[lead]), bytes * boxes(ahead.ks));
+                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[lead]), ahead.bytes * boxes(ahead.ks));
                     request(weights, SWAP, ahead, lead);
                 }
             grid_dependency_wait();
@@ -246,7 +266,7 @@ struct Roles {
             const bool ok = wait(&ctrl->empty[stage], phase ^ 1u, lane == 0 ? STATUS_TIMEOUT_PRODUCER : 0u, 0x50000000u | (stage << 16) | cursor.ks);
             if (!__all_sync(0xFFFFFFFFu, ok)) return;
             if (elect_one()) {
-                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[stage]), bytes * boxes(cursor.ks));
+                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[stage]), cursor.bytes * boxes(cursor.ks));
                 request(weights, SWAP, cursor, stage);
                 request(tokens, !SWAP, cursor, stage);
             }
@@ -260,13 +280,13 @@ struct Roles {
         constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
         // Instruction descriptor of kind::i8: 32-bit integer sums (2 at bit 4), A and B signed (1 at bits 7 and 10), both
         // K-major, N >> 3 at bit 17, M >> 4 at bit 24.
-        const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(g.width >> 3) << 17) | (uint32_t(128 * CG >> 4) << 24);
-        const uint32_t ring_lo = (smem & 0x3FFFFu) >> 4, y_pitch = uint32_t(g.width) * ROW_BYTES >> 4;
+        const uint32_t idesc_m = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 * CG >> 4) << 24);
+        const uint32_t ring_lo = (smem & 0x3FFFFu) >> 4, y_pitch = uint32_t(g.width / CG) * ROW_BYTES >> 4;
         int stage = 0;
         uint32_t phase = 0, iter = 0;
         bool landed = false;                                    // the probe of this stage's barrier succeeded
         for (Walk<CG, SWAP> walk(g, tile_start, row_start, unit, units); walk.valid(); walk.next(), ++iter) {
-            const uint32_t b = iter & 1u, acc = tmem + b * acc_stride;
+            const uint32_t b = iter & 1u, acc = tmem + b * acc_stride, idesc = idesc_m | (uint32_t(walk.tile().n >> 3) << 17);
             const bool free = wait(&ctrl->acc_free[b], ((iter >> 1) & 1u) ^ 1u, lane == 0 ? STATUS_TIMEOUT_MMA : 0u, 0x60000000u | iter);
             if (!__all_sync(0xFFFFFFFFu, free)) return;
             tc_fence_after_sync();
@@ -313,7 +333,7 @@ struct Roles {
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int column = half * 32 + c * 64 + lane;
-                across[c] = column < min(g.width, SWAP ? tokens : channels) ? __ldg(columns + column) : 0.0f;
+                across[c] = column < (SWAP ? tokens : min(g.width, channels)) ? __ldg(columns + column) : 0.0f;
             }
         }
     };
@@ -366,7 +386,7 @@ struct Roles {
             if (!__all_sync(0xFFFFFFFFu, ready)) return;
             tc_fence_after_sync();
             const uint32_t acc = tmem + b * acc_stride + (uint32_t(quarter * 32) << 16);
-            const int wide = SWAP ? min(g.width, t.token_end - t.token) : min(g.width, g.N - t.channel);     // the tile's columns
+            const int wide = SWAP ? t.token_end - t.token : min(g.width, g.N - t.channel);     // the tile's columns
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int column = half * 32 + c * 64;
@@ -401,7 +421,7 @@ struct Roles {
         const bool ready = wait(&ctrl->acc_full[0], 0u, lane == 0 ? STATUS_TIMEOUT_EPILOGUE : 0u, 0x71000000u);
         if (!__all_sync(0xFFFFFFFFu, ready)) return;
         tc_fence_after_sync();
-        const int wide = min(g.width, t.token_end - t.token), each = run_of(g.width, g.split), ch = quarter * 32 + lane;
+        const int wide = t.token_end - t.token, each = run_of(g.width, g.split), ch = quarter * 32 + lane;
         for (int column = half * 32; column < wide; column += 64) {
             uint32_t v[32];
             tmem_ld_32x32(tmem + (uint32_t(quarter * 32) << 16) + column, v);
@@ -421,7 +441,7 @@ struct Roles {
         Walk<CG, SWAP> walk(g, tile_start, row_start, unit, units);
         const Tile t = walk.tile();
         const int each = run_of(g.width, g.split), ch = thread % 128, channel = t.channel + ch;
-        const int first = int(rank) * each, count = min(each, min(g.width, t.token_end - t.token) - first);
+        const int first = int(rank) * each, count = min(each, t.token_end - t.token - first);
         const float sb = channel < g.N ? __ldg(g.b_scale + t.scale + ch) : 0.0f;
         by_out(g.out, [&](auto out) {
             constexpr int OUT = decltype(out)::value;
@@ -599,7 +619,8 @@ int resident(int device, int members) {
     return units;
 }
 int resident(const Int8Tiles& t, int device) {
-    return t.pair ? resident<2, false>(device, 2) : t.swap ? resident<1, true>(device, t.split) : resident<1, false>(device, 1);
+    if (t.pair) return t.swap ? resident<2, true>(device, 2) : resident<2, false>(device, 2);
+    return t.swap ? resident<1, true>(device, t.split) : resident<1, false>(device, 1);
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
@@ -634,13 +655,13 @@ float estimate(const Int8Tiles& t, int rows, int n, int k, int fit) {
 Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device) {
     Int8Tiles best{};
     if (experts) {
-        // By the mean number of rows: from 120 on CTA pairs (256 tokens a tile; 32 experts of 4096 x 4096, mean 192: 112
-        // us, 148 in the SWAP form), below as wide a tile as holds half as many again, so that most experts are one tile
-        // (mean 64: 96 columns 89 us, 64 columns 100, 128 columns 94).
+        // By the mean number of rows. From 64 on CTA pairs, whose SMs share the tokens of a tile (32 experts of 4096 x 4096,
+        // mean 128: 96 us, single CTAs 118; mean 64: 89 either way; 8 experts of 2048 x 2048, mean 32: 10.8 and 9.2). Below,
+        // as wide a tile as holds half as many rows again, so that most experts are one tile.
         const int mean = (rows + experts - 1) / experts;
-        best.pair = mean >= 120;
-        best.swap = !best.pair;
-        best.width = best.pair ? 256 : std::min(128, round_up(mean + mean / 2, 16));
+        best.pair = mean >= 64;
+        best.swap = 1;
+        best.width = best.pair ? 256 : mean <= 10 ? 16 : std::min(96, round_up(mean + mean / 2, 32));
         best.split = 1;
     } else {
         float best_ns = 0.0f;
@@ -673,11 +694,12 @@ void run(const int8_t* a, const int8_t* b, const float* a_scales, const float* b
     int device = 0;
     cuda_check(cudaGetDevice(&device));
     const Int8Tiles t = int8_tiles(M, N, K, experts, device);
-    // Boxes of the tokens' operand: no more rows than there are (rounded up to a swizzle group). What a stage holds beyond
-    // them is whatever was there: any byte is a number, a row of the product depends on its own row alone, and rows that do
-    // not exist are not stored.
-    const int x_tile = t.pair ? 256 : 128, y_rows_box = t.width / (t.pair ? 2 : 1), few = experts || t.pair ? 128 : round_up(M, 8);
-    const int x_box = t.swap ? 128 : std::min(128, few), y_box = t.swap && !experts ? std::min(y_rows_box, round_up(M, 8)) : y_rows_box;
+    // Boxes of the tokens' operand: no more rows than there are (rounded up to a swizzle group), in a grouped product 32 rows
+    // each. What a stage holds beyond them is whatever was there: any byte is a number, a row of the product depends on its
+    // own row alone, and rows that do not exist are not stored.
+    const int x_tile = t.pair ? 256 : 128, half = t.pair ? 2 : 1, few = round_up(M, 8);
+    const int x_box = t.swap || t.pair || experts ? 128 : std::min(128, few);
+    const int y_box = !t.swap ? t.width / half : experts ? std::min(32, t.width) : std::min(t.width, few);
     Args g{};
     g.M = M;
     g.N = N;
@@ -727,7 +749,8 @@ void run(const int8_t* a, const int8_t* b, const float* a_scales, const float* b
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = members > 1 ? 2 : 1;
-    if (t.pair) cuda_check(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<2, false>, tokens, weights, g));
+    if (t.pair && t.swap) cuda_check(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<2, true>, weights, tokens, g));
+    else if (t.pair) cuda_check(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<2, false>, tokens, weights, g));
     else if (t.swap) cuda_check(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<1, true>, weights, tokens, g));
     else cuda_check(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<1, false>, tokens, weights, g));
     g_launches.fetch_add(1, std::memory_order_relaxed);
