@@ -591,13 +591,16 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
 std::mutex g_lock;
 
 // CTAs (members = 1) or clusters of that many CTAs that are resident at once (one CTA per SM: its ring fills the shared
-// memory).
+// memory). 0 for a cluster the device has no room for.
 template <int CG, bool SWAP>
 int resident(int device, int members) {
-    static int cached[64][9] = {};
+    static std::atomic<int> cached[64][9] = {};
     const bool known = device >= 0 && device < 64;
+    if (known) {
+        const int units = cached[device][members].load(std::memory_order_acquire);         // one more than what fits
+        if (units) return units - 1;
+    }
     std::lock_guard<std::mutex> hold(g_lock);
-    if (known && cached[device][members]) return cached[device][members];
     auto kernel = int8_gemm_kernel<CG, SWAP>;
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
     int units = 0;
@@ -614,8 +617,8 @@ int resident(int device, int members) {
         cfg.numAttrs = 1;
         cuda_check(cudaOccupancyMaxActiveClusters(&units, kernel, &cfg));
     }
-    if (units < 1) throw std::runtime_error("int8 gemm: the kernel does not fit on this device");
-    if (known) cached[device][members] = units;
+    if (units < 1 && members <= 2) throw std::runtime_error("int8 gemm: the kernel does not fit on this device");
+    if (known) cached[device][members].store(units + 1, std::memory_order_release);
     return units;
 }
 int resident(const Int8Tiles& t, int device) {
@@ -637,13 +640,13 @@ size_t table_bytes(const Int8Tiles& t, int experts) {
 // both operands (130 bytes a ns) or what the instructions of a step cost, whichever is longest, and at least as long as
 // the weights need to arrive. The constants are a fit to 1949 timings (M = 1..4096, 11 shapes of N = 520..28672, K =
 // 1024..16384, all forms): what they pick is 0.2 % slower than the fastest on the mean, 4.6 % at worst.
-float estimate(const Int8Tiles& t, int rows, int n, int k, int fit) {
+float estimate(const Int8Tiles& t, int rows, int n, int k, int fit, int sms) {
     const int x = t.pair ? 256 : 128, x_rows = t.swap ? n : rows, y_rows = t.swap ? rows : n;
     const long long tiles = (long long)((x_rows + x - 1) / x) * ((y_rows + t.width - 1) / t.width), waves = (tiles + fit - 1) / fit;
     const int few = round_up(rows, 8), boxes = (k + ROW_BYTES - 1) / ROW_BYTES;
     const int taken = t.pair ? 128 + t.width / 2 : t.swap ? 128 + std::min(t.width, few) : std::min(128, few) + t.width;
     const float step = std::max({1.03f * float(t.width), float(taken * ROW_BYTES) / 130.0f, t.pair || t.swap ? 190.0f : 170.0f});
-    const int ctas = int(std::min(148ll, tiles * (t.pair ? 2 : t.split)));
+    const int ctas = int(std::min((long long)(sms), tiles * (t.pair ? 2 : t.split)));
     const float hbm = float(n) * float(k) / std::min(7930.0f, 92.5f * float(ctas));
     const float loop = float(waves) * float((boxes + t.split - 1) / t.split) * step;
     return 3100.0f + (t.pair ? 1100.0f : 0.0f) + std::max(hbm, loop) + 16.0f * float(t.width) + 1570.0f * float(waves - 1) +
@@ -665,15 +668,23 @@ Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device) {
         best.split = 1;
     } else {
         float best_ns = 0.0f;
+        const int sms = resident<1, false>(device, 1);
         auto consider = [&](int pair, int swap, int width, int split) {
             const Int8Tiles t{pair, swap, width, split, 0, 0};
-            const float ns = estimate(t, rows, n, k, resident(t, device));
+            const int fit = resident(t, device);
+            if (fit == 0) return;
+            const float ns = estimate(t, rows, n, k, fit, sms);
             if (best.width == 0 || ns < best_ns) { best = t; best_ns = ns; }
         };
         if (rows <= 128) {
             const int steps = (k + SUBS<1> * ROW_BYTES - 1) / (SUBS<1> * ROW_BYTES);
             for (int split = 1; split <= 8 && (split == 1 || steps / split >= 2); split *= 2) consider(0, 1, round_up(rows, 16), split);
-            for (int width = 16; width <= 256; width += 16) consider(0, 0, width, 1);
+            // as wide as it takes for one, two or three tiles per SM
+            for (int waves = 1, last = 0; waves <= 3; ++waves) {
+                const int width = std::min(256, round_up((n + waves * sms - 1) / (waves * sms), 16));
+                if (width != last) consider(0, 0, width, 1);
+                last = width;
+            }
         } else {
             for (int width = 32; width <= 256; width += 32) consider(1, 0, width, 1);
         }
