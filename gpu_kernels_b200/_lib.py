@@ -144,5 +144,18 @@ def on(device: torch.device):
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+def run(device: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with `device` current and its current stream, errors raised: what a short call spends on the two
+    context managers of `on` and `check` is a tenth of its time."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
+
+
 def launch_count() -> int:
     return int(load().gpu_kernels_nvfp4_launch_count())

@@ -25,19 +25,24 @@ def matrix(rows: int, columns: int, dtype: torch.dtype, device) -> torch.Tensor:
     return torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=device)
 
 
-def aligned(t: torch.Tensor) -> torch.Tensor:
-    """t, contiguous and on a 16-byte boundary: as it is where it is that already, else a copy."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def placed(t: torch.Tensor):
+    """(t, its address), t contiguous and on a 16-byte boundary: as it is where it is that already, else a copy."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    address = t.data_ptr()
+    if address % 16:
+        t = t.clone()
+        address = t.data_ptr()
+    return t, address
 
 
-def _rows(values: torch.Tensor, name: str) -> torch.Tensor:
+def _rows(values: torch.Tensor, name: str):
     _require_cuda(values, name)
     if values.dim() != 2:
         raise ValueError(f"{name} must be 2-D [rows, K]")
     if values.dtype not in _DTYPES:
         values = values.float()
-    return aligned(values.detach() if values.requires_grad else values)
+    return placed(values.detach() if values.requires_grad else values)
 
 
 def quantize_int8(values: torch.Tensor):
@@ -45,26 +50,24 @@ def quantize_int8(values: torch.Tensor):
 
     scale = max|row| / 127; a code is the integer nearest to 127 * value / max|row|, ties to the even one. A zero row has
     scale 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN."""
-    values = _rows(values, "values")
+    values, address = _rows(values, "values")
     rows, k = values.shape
-    codes = matrix(rows, k, torch.int8, values.device)
-    scales = torch.empty(rows, dtype=torch.float32, device=values.device)
-    with _lib.on(values.device):
-        _lib.check(_lib.load().gpu_kernels_int8_quantize(
-            values.data_ptr(), _DTYPES[values.dtype], codes.data_ptr(), scales.data_ptr(), rows, k, _lib.stream()))
+    device = values.device
+    codes = matrix(rows, k, torch.int8, device)
+    scales = torch.empty(rows, dtype=torch.float32, device=device)
+    _lib.run(device, _lib.load().gpu_kernels_int8_quantize, address, _DTYPES[values.dtype], codes.data_ptr(), scales.data_ptr(), rows, k)
     return codes, scales
 
 
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """codes * scales[:, None] -> fp32 [rows, K]."""
     _operand(codes, "codes", 2)
-    codes = aligned(codes)
+    codes, at_codes = placed(codes)
     rows, k = codes.shape
-    scales = _scales(scales, "scales", (rows,), codes.device)
-    out = matrix(rows, k, torch.float32, codes.device)
-    with _lib.on(codes.device):
-        _lib.check(_lib.load().gpu_kernels_int8_dequantize(
-            codes.data_ptr(), scales.data_ptr(), out.data_ptr(), rows, k, _lib.stream()))
+    device = codes.device
+    scales, at_scales = _scales(scales, "scales", (rows,), device)
+    out = matrix(rows, k, torch.float32, device)
+    _lib.run(device, _lib.load().gpu_kernels_int8_dequantize, at_codes, at_scales, out.data_ptr(), rows, k)
     return out
 
 
@@ -75,10 +78,10 @@ def _operand(t: torch.Tensor, name: str, dim: int, device=None) -> None:
         raise ValueError(f"{name} must be on {device}, where the other operands are")
 
 
-def _scales(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+def _scales(t: torch.Tensor, name: str, shape, device):
     if t.dtype != torch.float32 or t.shape != shape or t.device != device:
         raise ValueError(f"{name} must be an fp32 tensor of shape {tuple(shape)} on {device}")
-    return aligned(t)
+    return placed(t)
 
 
 def _output(out, m, n, dtype, device) -> torch.Tensor:
@@ -103,17 +106,16 @@ def int8_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales
     """C [M, N] = (a [M, K] @ b [N, K].T) * a_scales[:, None] * b_scales, in out's type (or out_dtype).
 
     Any M; N a multiple of 8, K a multiple of 16 up to 131056."""
+    device = a.device
     _operand(a, "a", 2)
-    _operand(b, "b", 2, a.device)
+    _operand(b, "b", 2, device)
     (m, k), (n, k2) = a.shape, b.shape
     _check_sizes(n, k, k2)
-    a, b = aligned(a), aligned(b)
-    a_scales, b_scales = _scales(a_scales, "a_scales", (m,), a.device), _scales(b_scales, "b_scales", (n,), a.device)
-    out = _output(out, m, n, out_dtype, a.device)
-    with _lib.on(a.device):
-        _lib.check(_lib.load().gpu_kernels_int8_gemm(
-            a.data_ptr(), b.data_ptr(), a_scales.data_ptr(), b_scales.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], m, n, k,
-            _lib.stream()))
+    (a, at_a), (b, at_b) = placed(a), placed(b)
+    a_scales, at_a_scales = _scales(a_scales, "a_scales", (m,), device)
+    b_scales, at_b_scales = _scales(b_scales, "b_scales", (n,), device)
+    out = _output(out, m, n, out_dtype, device)
+    _lib.run(device, _lib.load().gpu_kernels_int8_gemm, at_a, at_b, at_a_scales, at_b_scales, out.data_ptr(), _DTYPES[out.dtype], m, n, k)
     return out
 
 
@@ -122,19 +124,18 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
     """x [M, K] (bf16, fp16 or fp32), quantised token by token, times weight [N, K] int8 -> [M, N] in x's type (or
     out_dtype): int8_gemm(*quantize_int8(x), ...) in one call. The product requests its first weights while the quantiser
     runs."""
-    x = _rows(x, "x")
-    _operand(weight, "weight", 2, x.device)
+    x, at_x = _rows(x, "x")
+    device, dtype = x.device, x.dtype
+    _operand(weight, "weight", 2, device)
     (m, k), (n, k2) = x.shape, weight.shape
     _check_sizes(n, k, k2)
-    weight = aligned(weight)
-    weight_scales = _scales(weight_scales, "weight_scales", (n,), x.device)
-    out = _output(out, m, n, out_dtype or x.dtype, x.device)
-    room = torch.empty(m * (k + 4), dtype=torch.uint8, device=x.device)             # the codes, then the tokens' scales
+    weight, at_weight = placed(weight)
+    weight_scales, at_scales = _scales(weight_scales, "weight_scales", (n,), device)
+    out = _output(out, m, n, out_dtype or dtype, device)
+    room = torch.empty(m * (k + 4), dtype=torch.uint8, device=device)               # the codes, then the tokens' scales
     codes = room.data_ptr()
-    with _lib.on(x.device):
-        _lib.check(_lib.load().gpu_kernels_int8_linear(
-            x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), weight_scales.data_ptr(), codes, codes + m * k, out.data_ptr(),
-            _DTYPES[out.dtype], m, n, k, _lib.stream()))
+    _lib.run(device, _lib.load().gpu_kernels_int8_linear, at_x, _DTYPES[dtype], at_weight, at_scales, codes, codes + m * k,
+             out.data_ptr(), _DTYPES[out.dtype], m, n, k)
     return out
 
 
@@ -154,15 +155,14 @@ def int8_grouped_gemm(rows: torch.Tensor, weights: torch.Tensor, row_scales: tor
         raise ValueError("1..1024 experts")
     if offsets.dtype != torch.int32 or offsets.shape != (experts + 1,) or offsets.device != rows.device:
         raise ValueError(f"offsets must be an int32 tensor of {experts + 1} values on {rows.device}")
-    rows, weights, offsets = aligned(rows), aligned(weights), offsets.contiguous()
-    row_scales = _scales(row_scales, "row_scales", (r,), rows.device)
-    weight_scales = _scales(weight_scales, "weight_scales", (experts, n), rows.device)
+    device = rows.device
+    (rows, at_rows), (weights, at_weights), offsets = placed(rows), placed(weights), offsets.contiguous()
+    row_scales, at_row_scales = _scales(row_scales, "row_scales", (r,), device)
+    weight_scales, at_weight_scales = _scales(weight_scales, "weight_scales", (experts, n), device)
     made = out is None
-    out = _output(out, r, n, out_dtype, rows.device)
-    with _lib.on(rows.device):
-        _lib.check(_lib.load().gpu_kernels_int8_grouped_gemm(
-            rows.data_ptr(), weights.data_ptr(), row_scales.data_ptr(), weight_scales.data_ptr(), offsets.data_ptr(), experts,
-            out.data_ptr(), _DTYPES[out.dtype], r, n, k, 1 if made else 0, _lib.stream()))
+    out = _output(out, r, n, out_dtype, device)
+    _lib.run(device, _lib.load().gpu_kernels_int8_grouped_gemm, at_rows, at_weights, at_row_scales, at_weight_scales,
+             offsets.data_ptr(), experts, out.data_ptr(), _DTYPES[out.dtype], r, n, k, 1 if made else 0)
     return out
 
 

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .int8 import aligned, matrix
+from .int8 import matrix, placed
 from .nvfp4 import _DTYPES, _require_cuda
 
 
@@ -48,10 +48,8 @@ def sort_routes(ids: torch.Tensor, num_experts: int) -> Routes:
     lib = _lib.load()
     needed = lib.gpu_kernels_tokens_sort_workspace(routes, num_experts)
     room = torch.empty(needed, dtype=torch.uint8, device=d) if needed else None
-    with _lib.on(d):
-        _lib.check(lib.gpu_kernels_tokens_sort(
-            ids.data_ptr(), ids.element_size(), routes, num_experts, offsets.data_ptr(), position.data_ptr(), source.data_ptr(),
-            None if room is None else room.data_ptr(), _lib.stream()))
+    _lib.run(d, lib.gpu_kernels_tokens_sort, ids.data_ptr(), ids.element_size(), routes, num_experts, offsets.data_ptr(),
+             position.data_ptr(), source.data_ptr(), None if room is None else room.data_ptr())
     return Routes(offsets, position, source)
 
 
@@ -78,21 +76,20 @@ def _values(t: torch.Tensor, name: str) -> torch.Tensor:
 def _gather(x, routes):
     x = x.contiguous()
     position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
-    rows = matrix(tokens * topk, x.shape[1], x.dtype, x.device)
-    with _lib.on(x.device):
-        _lib.check(_lib.load().gpu_kernels_tokens_gather(
-            x.data_ptr(), _DTYPES[x.dtype], tokens, topk, x.shape[1], position, live, rows.data_ptr(), _lib.stream()))
+    hidden = x.shape[1]
+    rows = matrix(tokens * topk, hidden, x.dtype, x.device)
+    _lib.run(x.device, _lib.load().gpu_kernels_tokens_gather, x.data_ptr(), _DTYPES[x.dtype], tokens, topk, hidden, position, live,
+             rows.data_ptr())
     return rows
 
 
 def _combine(rows, routes, weights):
     rows = rows.contiguous()
     position, live, tokens, topk = _check_routes(routes, None, rows.device)
-    y = matrix(tokens, rows.shape[1], rows.dtype, rows.device)
-    with _lib.on(rows.device):
-        _lib.check(_lib.load().gpu_kernels_tokens_combine(
-            rows.data_ptr(), _DTYPES[rows.dtype], None if weights is None else weights.data_ptr(), position, live, tokens, topk,
-            rows.shape[1], y.data_ptr(), _lib.stream()))
+    hidden = rows.shape[1]
+    y = matrix(tokens, hidden, rows.dtype, rows.device)
+    _lib.run(rows.device, _lib.load().gpu_kernels_tokens_combine, rows.data_ptr(), _DTYPES[rows.dtype],
+             None if weights is None else weights.data_ptr(), position, live, tokens, topk, hidden, y.data_ptr())
     return y
 
 
@@ -129,11 +126,9 @@ class _CombineTokens(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             d_weights = matrix(tokens, topk, torch.float32, d_y.device)
             rows = rows.contiguous()
-        with _lib.on(d_y.device):
-            _lib.check(_lib.load().gpu_kernels_tokens_combine_backward(
-                d_y.data_ptr(), _DTYPES[d_y.dtype], None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live,
-                tokens, topk, d_y.shape[1], None if d_rows is None else d_rows.data_ptr(),
-                None if d_weights is None else d_weights.data_ptr(), _lib.stream()))
+        _lib.run(d_y.device, _lib.load().gpu_kernels_tokens_combine_backward, d_y.data_ptr(), _DTYPES[d_y.dtype],
+                 None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live, tokens, topk, d_y.shape[1],
+                 None if d_rows is None else d_rows.data_ptr(), None if d_weights is None else d_weights.data_ptr())
         return d_rows, d_weights, None
 
 
@@ -150,16 +145,15 @@ def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
 def gather_tokens_int8(x: torch.Tensor, routes: Routes):
     """quantize_int8(x) in the order of the routes: x [T, K] -> (codes int8 [T * topk, K], scales fp32 [T * topk]), the rows
     `int8_grouped_gemm` takes. A token is quantised once, K a multiple of 16; rows of no expert have codes and scale 0."""
-    x = aligned(_values(x, "x"))
+    x, at_x = placed(_values(x, "x"))
     position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
     k = x.shape[1]
     if k % 16:
         raise ValueError("K must be a multiple of 16")
     codes = matrix(tokens * topk, k, torch.int8, x.device)
     scales = torch.empty(tokens * topk, dtype=torch.float32, device=x.device)
-    with _lib.on(x.device):
-        _lib.check(_lib.load().gpu_kernels_tokens_gather_int8(
-            x.data_ptr(), _DTYPES[x.dtype], tokens, topk, k, position, live, codes.data_ptr(), scales.data_ptr(), _lib.stream()))
+    _lib.run(x.device, _lib.load().gpu_kernels_tokens_gather_int8, at_x, _DTYPES[x.dtype], tokens, topk, k, position, live,
+             codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
