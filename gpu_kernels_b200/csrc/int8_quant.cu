@@ -197,19 +197,21 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
 // the next row takes each value's own scale.
 constexpr int DEQUANT_GROUPS = 4;                               // groups per thread, a block's threads apart
 
+// Index: 32 bits wide where the number of values allows (a 64-bit division for each group took 59 us).
+template <typename Index>
 __global__ void __launch_bounds__(256)
 int8_dequantise_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, float* __restrict__ out, size_t values, int K) {
     ptx::chain_point();
-    const size_t first = size_t(blockIdx.x) * (256 * DEQUANT_GROUPS) + threadIdx.x, groups = values / 4;
+    const Index first = Index(blockIdx.x) * (256 * DEQUANT_GROUPS) + threadIdx.x, groups = Index(values / 4);
     char4 c[DEQUANT_GROUPS];
     #pragma unroll
     for (int j = 0; j < DEQUANT_GROUPS; ++j)
         if (first + j * 256 < groups) c[j] = __ldg(reinterpret_cast<const char4*>(codes) + first + j * 256);
     #pragma unroll
     for (int j = 0; j < DEQUANT_GROUPS; ++j) {
-        const size_t group = first + j * 256;
+        const Index group = first + j * 256;
         if (group >= groups) continue;
-        const size_t row = group * 4 / uint32_t(K);
+        const Index row = group * 4 / uint32_t(K);
         const uint32_t column = uint32_t(group * 4 - row * uint32_t(K));
         float s[4];
         s[0] = s[1] = s[2] = s[3] = __ldg(scales + row);
@@ -220,7 +222,7 @@ int8_dequantise_kernel(const int8_t* __restrict__ codes, const float* __restrict
         reinterpret_cast<float4*>(out)[group] = make_float4(float(c[j].x) * s[0], float(c[j].y) * s[1], float(c[j].z) * s[2], float(c[j].w) * s[3]);
     }
     if (blockIdx.x == 0 && threadIdx.x < values % 4) {          // what is left behind the last group
-        const size_t i = groups * 4 + threadIdx.x;
+        const size_t i = values / 4 * 4 + threadIdx.x;
         out[i] = float(codes[i]) * __ldg(scales + i / uint32_t(K));
     }
 }
@@ -298,7 +300,8 @@ void int8_dequantise(const int8_t* codes, const float* scales, float* out, long 
         throw std::invalid_argument("int8 dequantise: codes and out must be 16-byte aligned");
     const size_t values = size_t(rows) * K, blocks = (values + 4 * 256 * DEQUANT_GROUPS - 1) / (4 * 256 * DEQUANT_GROUPS);
     if (blocks > 0x7FFFFFFFull) throw std::invalid_argument("int8 dequantise: too many values");
-    launch_chained(int8_dequantise_kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, codes, scales, out, values, K);
+    auto kernel = values < (size_t(1) << 31) ? int8_dequantise_kernel<uint32_t> : int8_dequantise_kernel<size_t>;
+    launch_chained(kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, codes, scales, out, values, K);
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 

@@ -253,6 +253,26 @@ def test_grouped_offsets_that_make_no_sense_stay_in_bounds(g):
     assert_product(c, reference_grouped(rows, weights, sr, sw, [0, 20, 20, 50, 50]))
 
 
+def test_matrices_beyond_31_bits(g):
+    # 70001 x 30728 values: the last rows lie behind element 2^31
+    rows, k, tail = 70001, 30728, slice(69990, None)
+    x = torch.empty((rows, k), dtype=BF16, device="cuda").normal_(generator=generator(1))
+    codes, scales = g.quantize_int8(x)
+    want, want_scales = codes_of(x[tail])
+    del x
+    assert torch.equal(codes[tail], want) and torch.equal(scales[tail], want_scales)
+    assert torch.equal(g.dequantize_int8(codes, scales)[tail], codes[tail].float() * scales[tail, None])
+    del codes
+    a, b = random_codes((rows, 32), 2), random_codes((k, 32), 3)
+    sa, sb = random_scales((rows,), 4), random_scales((k,), 5)
+    assert_product(g.int8_gemm(a, b, sa, sb)[tail], exact(a[tail], b, sa[tail], sb))
+    offsets = torch.tensor([0, 30000, 69995, 70001], dtype=torch.int32, device="cuda")
+    b3, sb3 = torch.stack((b, b, b.flip(0))), torch.stack((sb, sb, sb.flip(0)))
+    c = g.int8_grouped_gemm(a, b3, sa, sb3, offsets)
+    assert_product(c[69990:69995], exact(a[69990:69995], b, sa[69990:69995], sb))
+    assert_product(c[69995:], exact(a[69995:], b.flip(0), sa[69995:], sb.flip(0)))
+
+
 def test_no_rows(g):
     b, sb = random_codes((16, 32), 1), random_scales((16,), 1)
     assert g.int8_gemm(random_codes((0, 32), 1), b, random_scales((0,), 1), sb).shape == (0, 16)

@@ -45,3 +45,29 @@ def test_nvfp4_linears_in_a_row(g):
         p.validate()
         p.close()
     assert all(torch.equal(a, b) for a, b in zip(last, want))
+
+
+@pytest.mark.timeout(60)
+def test_two_streams_at_once(g):
+    # products of both kinds, on pairs and on single CTAs, with nothing between the streams
+    x = [torch.randn((m, 4096), device="cuda").bfloat16() for m in (600, 8)]
+    w, ws = g.quantize_int8(torch.randn((4096, 4096), device="cuda").bfloat16())
+    b, sb = g.quantize(torch.randn((4096, 4096), device="cuda").bfloat16())
+    plans = [g.Nvfp4Gemm(*(lambda q: (q[0], b, q[1], sb))(g.quantize(v))) for v in x]
+    ids = torch.randint(0, 64, (4000, 4), device="cuda")
+    calls = [lambda: g.int8_linear(x[0], w, ws), lambda: plans[0].linear(x[0]), lambda: g.int8_linear(x[1], w, ws),
+             lambda: g.sort_routes(ids, 64).source]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [None] * len(calls)
+    for _ in range(100):
+        for i, (call, stream) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(stream):
+                got[i] = call()
+    torch.cuda.synchronize()
+    g.check_int8()
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+    for plan in plans:
+        plan.close()

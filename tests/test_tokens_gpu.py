@@ -186,6 +186,21 @@ def test_gather_quantised(g, tokens, topk, experts, k, dtype):
     assert torch.equal(scales[routes.position.long()], torch.where(live, token_scales[:, None], 0.0))
 
 
+def test_rows_beyond_31_bits(g):
+    # 9000 tokens of eight routes, 30728 values a row: the last rows lie behind element 2^31
+    tokens, topk, experts, hidden = 9000, 8, 16, 30728
+    routes = g.sort_routes(choices(tokens, topk, experts, 1), experts)
+    x = torch.empty((tokens, hidden), dtype=BF16, device="cuda").normal_(generator=generator(2)).requires_grad_()
+    rows = g.gather_tokens(x, routes)
+    token = routes.source.long() // topk
+    assert torch.equal(rows[-50:], x.detach()[token[-50:]])
+    w = torch.full((tokens, topk), 0.125, device="cuda")
+    y = g.combine_tokens(rows, routes, w)                        # eight times an eighth of each value: exact
+    assert torch.equal(y, x)
+    d_x, = torch.autograd.grad(y, x, x.detach())
+    assert torch.equal(d_x, x)
+
+
 def test_positions_outside_the_rows_are_skipped(g):
     # an order of the caller's own making: nothing is read or written out of bounds
     d = torch.device("cuda")
