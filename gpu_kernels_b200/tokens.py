@@ -53,8 +53,13 @@ def sort_routes(ids: torch.Tensor, num_experts: int) -> Routes:
     return Routes(offsets, position, source)
 
 
+def _places(position: torch.Tensor, offsets: torch.Tensor) -> tuple[int, int, int, int]:
+    """The addresses of the positions and of the number of live rows, tokens, topk."""
+    return (position.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), *position.shape)
+
+
 def _check_routes(routes: Routes, tokens: int | None, device) -> tuple[int, int, int, int]:
-    """(position, live rows, tokens, topk) of a checked order, the first two as device addresses."""
+    """The places of a checked order."""
     offsets, position = routes.offsets, routes.position
     if position.dim() != 2 or position.shape[1] < 1 or (tokens is not None and position.shape[0] != tokens):
         raise ValueError("the routes are not those of this many tokens")
@@ -63,7 +68,7 @@ def _check_routes(routes: Routes, tokens: int | None, device) -> tuple[int, int,
             raise ValueError(f"routes.{name} must be a contiguous int32 tensor on {device}")
     if offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError("routes.offsets must hold one value per expert and one more")
-    return position.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), position.shape[0], position.shape[1]
+    return _places(position, offsets)
 
 
 def _values(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -73,9 +78,9 @@ def _values(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _gather(x, routes):
+def _gather(x, places):
     x = x.contiguous()
-    position, live, tokens, topk = _check_routes(routes, x.shape[0], x.device)
+    position, live, tokens, topk = places
     hidden = x.shape[1]
     rows = matrix(tokens * topk, hidden, x.dtype, x.device)
     _lib.run(x.device, _lib.load().gpu_kernels_tokens_gather, x.data_ptr(), _DTYPES[x.dtype], tokens, topk, hidden, position, live,
@@ -83,9 +88,9 @@ def _gather(x, routes):
     return rows
 
 
-def _combine(rows, routes, weights):
+def _combine(rows, places, weights):
     rows = rows.contiguous()
-    position, live, tokens, topk = _check_routes(routes, None, rows.device)
+    position, live, tokens, topk = places
     hidden = rows.shape[1]
     y = matrix(tokens, hidden, rows.dtype, rows.device)
     _lib.run(rows.device, _lib.load().gpu_kernels_tokens_combine, rows.data_ptr(), _DTYPES[rows.dtype],
@@ -95,41 +100,42 @@ def _combine(rows, routes, weights):
 
 class _GatherTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, routes):
-        ctx.save_for_backward(*routes)
-        return _gather(x, routes)
+    def forward(ctx, x, position, offsets, places):
+        ctx.save_for_backward(position, offsets)
+        return _gather(x, places)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_rows):
-        return _combine(d_rows, Routes(*ctx.saved_tensors), None), None
+        return _combine(d_rows, _places(*ctx.saved_tensors), None), None, None, None
 
 
 class _CombineTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, routes):
-        ctx.save_for_backward(rows if weights is not None and ctx.needs_input_grad[1] else None, weights, *routes)
-        return _combine(rows, routes, weights)
+    def forward(ctx, rows, weights, position, offsets, places):
+        ctx.save_for_backward(position, offsets, weights, rows if weights is not None and ctx.needs_input_grad[1] else None)
+        return _combine(rows, places, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_y):
-        rows, weights, *order = ctx.saved_tensors
-        routes = Routes(*order)
+        position, offsets, weights, rows = ctx.saved_tensors
+        places = _places(position, offsets)
         if weights is None:
-            return _gather(d_y, routes), None, None
+            return _gather(d_y, places), None, None, None, None
+        position, live, tokens, topk = places
         d_y = d_y.contiguous()
-        position, live, tokens, topk = _check_routes(routes, d_y.shape[0], d_y.device)
+        hidden = d_y.shape[1]
         d_rows = d_weights = None
         if ctx.needs_input_grad[0]:
-            d_rows = matrix(tokens * topk, d_y.shape[1], d_y.dtype, d_y.device)
+            d_rows = matrix(tokens * topk, hidden, d_y.dtype, d_y.device)
         if ctx.needs_input_grad[1]:
             d_weights = matrix(tokens, topk, torch.float32, d_y.device)
             rows = rows.contiguous()
         _lib.run(d_y.device, _lib.load().gpu_kernels_tokens_combine_backward, d_y.data_ptr(), _DTYPES[d_y.dtype],
-                 None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live, tokens, topk, d_y.shape[1],
+                 None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live, tokens, topk, hidden,
                  None if d_rows is None else d_rows.data_ptr(), None if d_weights is None else d_weights.data_ptr())
-        return d_rows, d_weights, None
+        return d_rows, d_weights, None, None, None
 
 
 def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
@@ -137,9 +143,10 @@ def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
 
     Gradient: x's is the sum of its live rows' gradients, in FP32 and the order of the routes, rounded once."""
     _values(x, "x")
+    places = _check_routes(routes, x.shape[0], x.device)
     if x.requires_grad and torch.is_grad_enabled():
-        return _GatherTokens.apply(x, routes)
-    return _gather(x, routes)
+        return _GatherTokens.apply(x, routes.position, routes.offsets, places)
+    return _gather(x, places)
 
 
 def gather_tokens_int8(x: torch.Tensor, routes: Routes):
@@ -169,6 +176,7 @@ def combine_tokens(rows: torch.Tensor, routes: Routes, weights: torch.Tensor | N
         if weights.shape != routes.position.shape or weights.device != rows.device or not weights.is_floating_point():
             raise ValueError("weights must be floating-point, [tokens, topk] and where the rows are")
         weights = weights.float().contiguous()
+    places = _check_routes(routes, None, rows.device)
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
-        return _CombineTokens.apply(rows, weights, routes)
-    return _combine(rows, routes, weights)
+        return _CombineTokens.apply(rows, weights, routes.position, routes.offsets, places)
+    return _combine(rows, places, weights)
