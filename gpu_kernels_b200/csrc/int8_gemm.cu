@@ -65,6 +65,7 @@ struct Args {
     const float* b_scale;
     uint8_t* c;
     int out;                        // InputDtype of C
+    int rows_32;                    // every row of C starts on a 32-byte boundary
     const int* offsets;             // grouped: [experts + 1]; null = dense
     int experts;
     int zero_rest;                  // grouped: rows of C behind the last expert's are cleared
@@ -337,24 +338,31 @@ struct Roles {
             }
         }
     };
-    // 32 accumulator columns of one lane. Tokens on the lanes: 32 channels of one row of C.
+    // 32 accumulator columns of one lane. Tokens on the lanes: 32 channels of one row of C, in 32-byte stores where every
+    // row starts on a 32-byte boundary (16-byte ones write each sector of C in two halves).
     template <int OUT>
     __device__ __forceinline__ void store_row(const uint32_t (&v)[32], const Tile& t, int token, float own, float across, int column, int wide) const {
-        uint8_t* row = g.c + (size_t(token) * g.N + t.channel + column) * (OUT == DTYPE_F32 ? 4 : 2);
-        const int count = token < t.token_end ? wide - column : 0;
+        constexpr int SIZE = OUT == DTYPE_F32 ? 4 : 2, PER = 32 / SIZE;          // values in 32 bytes
+        uint8_t* row = g.c + (size_t(token) * g.N + t.channel + column) * SIZE;
+        const int count = token < t.token_end ? wide - column : 0;               // a multiple of 8, of 16 with rows_32 and 16-bit values
         #pragma unroll
-        for (int q = 0; q < 4; ++q) {                           // N is a multiple of 8: eight channels are there or not
-            float f[8];
+        for (int q = 0; q < 32 / PER; ++q) {
+            uint32_t w[8];
             #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = scaled(v[8 * q + i], own, __shfl_sync(0xFFFFFFFFu, across, 8 * q + i));
-            if (8 * q >= count) continue;
-            if constexpr (OUT == DTYPE_F32) {
-                float4* dst = reinterpret_cast<float4*>(row) + 2 * q;
-                dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-                dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+            for (int i = 0; i < 8; ++i) {
+                const int at = q * PER + i * (4 / SIZE);
+                const float f = scaled(v[at], own, __shfl_sync(0xFFFFFFFFu, across, at));
+                if constexpr (OUT == DTYPE_F32) w[i] = __float_as_uint(f);
+                else w[i] = pack_pair<OUT>(f, scaled(v[at + 1], own, __shfl_sync(0xFFFFFFFFu, across, at + 1)));
+            }
+            uint8_t* dst = row + q * 32;
+            if (g.rows_32) {
+                if (q * PER < count)
+                    asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                                 :: "l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
             } else {
-                reinterpret_cast<uint4*>(row)[q] =
-                    make_uint4(pack_pair<OUT>(f[0], f[1]), pack_pair<OUT>(f[2], f[3]), pack_pair<OUT>(f[4], f[5]), pack_pair<OUT>(f[6], f[7]));
+                if (q * PER < count) reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (q * PER + PER / 2 < count) reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
             }
         }
     }
@@ -726,6 +734,7 @@ void run(const int8_t* a, const int8_t* b, const float* a_scales, const float* b
     g.b_scale = b_scales;
     g.c = static_cast<uint8_t*>(C);
     g.out = out_dtype;
+    g.rows_32 = reinterpret_cast<uintptr_t>(C) % 32 == 0 && size_t(N) * dtype_bytes(out_dtype) % 32 == 0 ? 1 : 0;
     g.offsets = offsets;
     g.experts = experts;
     g.zero_rest = zero_rest ? 1 : 0;
