@@ -20,9 +20,9 @@
 //     one width for all, 256 experts of unequal popularity took 1143 us instead of 891 in a loop (4096 tokens of six
 //     routes). A tile that reaches into the next expert's rows (or channels) computes them with the wrong weights and does
 //     not store them.
-// Measured: 8192 cubed 331 us (3.32 POPS, twice the rate cuBLAS reaches in bf16); 1 x 8192 x 8192 15.2 us (4.4 TB/s), 1 x
-// 28672 x 8192 40.4 us (5.8 TB/s), 128 x 28672 x 8192 44 us; 256 experts of 4096 x 4096 with 64 tokens of six routes each
-// 470 us (7.1 TB/s).
+// Measured: 8192 cubed 326 us (3.37 POPS, twice the rate cuBLAS reaches in bf16; 359 under the power cap); 1 x 8192 x 8192
+// 15.2 us (4.4 TB/s), 1 x 28672 x 8192 40.4 us (5.8 TB/s), 128 x 28672 x 8192 44 us; 256 experts of 4096 x 4096 with 64
+// tokens of six routes each 470 us (7.1 TB/s).
 #include "operators_internal.h"
 #include "ptx.cuh"
 

@@ -5,7 +5,8 @@
 // amax = 2x, for example, 127 x / amax is 63.5): see code_of. A zero row has scale 0 and codes 0. A row that holds a NaN
 // or an infinity has scale NaN and codes 0: what is computed from it is NaN, not a number that looks sound.
 //
-// HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes. Threads take 16
+// HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes (8192 x 8192 bf16
+// 31.6 us, 6.4 TB/s; FP32 52 us; 8192 x 8191 bf16 34.7). Threads take 16
 // values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
 // and stores are aligned whatever K is; what a row has in front of its first whole group and behind its last one (up to 15
 // values each) is taken by 32 threads, one value each.
@@ -193,7 +194,7 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
 }
 
 // The codes of all rows as one flat array, four to a thread at a time: a warp reads 128 bytes and writes 512, both in one
-// run (with sixteen codes and four 16-byte stores to a thread 8192 x 8192 took 76 us). A group of four that reaches into
+// run: 8192 x 8192 51.9 us, 6.5 TB/s (with sixteen codes and four 16-byte stores to a thread 76). A group of four that reaches into
 // the next row takes each value's own scale.
 constexpr int DEQUANT_GROUPS = 4;                               // groups per thread, a block's threads apart
 
