@@ -68,7 +68,7 @@ struct Args {
     int rows_32;                    // every row of C starts on a 32-byte boundary
     const int* offsets;             // grouped: [experts + 1]; null = dense
     int experts;
-    int zero_rest;                  // grouped: rows of C behind the last expert's are cleared
+    int zero_rest;                  // grouped: rows of C that are no expert's are cleared
     int early;                      // the weights may be read before the grid in front of this one has finished
     uint32_t* status;
 };
@@ -85,8 +85,8 @@ struct Tile {
 template <int CG, bool SWAP>
 struct Walk {
     const Args& g;
-    const int* tile_start;          // grouped: first tile and first row of every expert, [experts + 1] each
-    const int* row_start;
+    const int* tile_start;          // grouped: first tile of every expert and their number, [experts + 1]
+    const int* row_start;           // grouped: first row of every expert and first row behind, [experts][2]
     int t, stride, tiles, expert;
     __device__ Walk(const Args& args, const int* ts, const int* rs, int unit, int units)
         : g(args), tile_start(ts), row_start(rs), t(unit), stride(units), expert(0) {

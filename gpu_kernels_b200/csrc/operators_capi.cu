@@ -72,7 +72,8 @@ int gpu_kernels_int8_grouped_gemm(const void* rows, const void* weights, const v
 
 int gpu_kernels_int8_tiles(int rows, int N, int K, int experts, int* info) {
     return guarded([&] {
-        if (!info || rows < 1 || N < 1 || K < 1 || experts < 0) throw std::invalid_argument("int8 tiles: positive sizes and an output");
+        if (!info || rows < 1 || N < 1 || K < 1 || experts < 0 || rows > 1 << 30 || N > 1 << 30 || experts > 1024)
+            throw std::invalid_argument("int8 tiles: positive sizes (rows and N up to 2^30, 1024 experts) and an output");
         int device = 0;
         cuda_check(cudaGetDevice(&device));
         const Int8Tiles t = int8_tiles(rows, N, K, experts, device);
