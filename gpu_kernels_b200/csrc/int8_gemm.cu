@@ -8,11 +8,12 @@
 // and 6-9, two per Tensor Memory lane quarter, drain the accumulators. Two accumulators take turns, so that a tile is
 // drained while the next one is computed. The forms, all persistent but the split one:
 //   CTA pairs: 256 tokens on the MMA's M side, up to 256 channels on its N side. For many tokens: bound by the tensor cores.
-//   Single CTAs: the same with up to 128 tokens and as many channels to a tile (in steps of 16) as give each SM one tile.
+//   Single CTAs: the same with 128 tokens and as many channels to a tile (in steps of 16) as give each SM one tile.
 //   SWAP, single CTAs: 128 channels on the M side, the tokens on the N side, in as narrow a tile as holds them. For few
-//     tokens, where each weight byte is read once and HBM is the bound. Where the tiles are fewer than the SMs, a cluster of
-//     2, 4 or 8 CTAs shares a tile's K loop: their integer partial sums meet in distributed shared memory, and the order in
-//     which they are added does not matter.
+//     tokens, where each weight byte is read once and HBM is the bound.
+//   Either kind of single CTAs, where the tiles are fewer than the SMs: a cluster of 2, 4 or 8 CTAs shares a tile's K loop.
+//     Their integer partial sums meet in distributed shared memory, and the order in which they are added does not matter
+//     (1022 x 1024 x 12880 27.7 us, with the widths of pairs alone 32.4; 128 x 8192 x 8192 16.6 and 19.1).
 //   Grouped, SWAP, single CTAs or pairs (256 channels): rows sorted by expert, `offsets` (device) says where each expert's
 //     rows start, the weights are stacked [experts, N, K]. Every CTA counts the experts' tiles once and walks the same
 //     sequence, an expert's tokens innermost, so that its weights are read from HBM once. An expert's rows are dealt evenly
@@ -417,19 +418,20 @@ struct Roles {
         }
     }
 
-    // One tile whose K loop the cluster shares. The tile's columns (tokens) are dealt to the CTAs in runs of `each`; a CTA has
-    // room for its run of every member's partial sums, [split][each / 4][128 channels][4 columns], so that lanes send and
-    // read 16 bytes in a row.
-    __device__ void send(uint32_t tmem, uint32_t room, float* token_scale, int quarter, int half, int lane) const {
+    // One tile whose K loop the cluster shares. The tile's columns are dealt to the CTAs in runs of `each`; a CTA has room for
+    // its run of every member's partial sums, [split][each / 4][128 lanes][4 columns], so that lanes send and read 16 bytes
+    // in a row.
+    __device__ __forceinline__ int columns_of(const Tile& t) const { return SWAP ? t.token_end - t.token : min(g.width, g.N - t.channel); }
+    __device__ void send(uint32_t tmem, uint32_t room, float* column_scale, int quarter, int half, int lane) const {
         if (g.early) grid_dependency_wait();
         Walk<CG, SWAP> walk(g, tile_start, row_start, unit, units);
         const Tile t = walk.tile();
-        const int thread = (half * 4 + quarter) * 32 + lane;    // (at least as many as columns)
-        token_scale[thread] = t.token + thread < t.token_end ? __ldg(g.a_scale + t.token + thread) : 0.0f;
+        const int thread = (half * 4 + quarter) * 32 + lane, wide = columns_of(t);          // (at least as many threads as columns)
+        column_scale[thread] = thread < wide ? __ldg(SWAP ? g.a_scale + t.token + thread : g.b_scale + t.scale + thread) : 0.0f;
         const bool ready = wait(&ctrl->acc_full[0], 0u, lane == 0 ? STATUS_TIMEOUT_EPILOGUE : 0u, 0x71000000u);
         if (!__all_sync(0xFFFFFFFFu, ready)) return;
         tc_fence_after_sync();
-        const int wide = t.token_end - t.token, each = run_of(g.width, g.split), ch = quarter * 32 + lane;
+        const int each = run_of(g.width, g.split), on_lane = quarter * 32 + lane;
         for (int column = half * 32; column < wide; column += 64) {
             uint32_t v[32];
             tmem_ld_32x32(tmem + (uint32_t(quarter * 32) << 16) + column, v);
@@ -438,33 +440,42 @@ struct Roles {
             #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 if (column + i >= wide) break;
-                const uint32_t at = room + uint32_t(((int(rank) * (each / 4) + group) * 128 + ch) * 16);
+                const uint32_t at = room + uint32_t(((int(rank) * (each / 4) + group) * 128 + on_lane) * 16);
                 asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};"
                              :: "r"(map_to_cta(at, uint32_t(owner))), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]) : "memory");
                 if (++group == each / 4) { group = 0; ++owner; }
             }
         }
     }
-    __device__ void finish(const int4* room, const float* token_scale, int thread) const {
+    __device__ void finish(const int4* room, const float* column_scale, int thread) const {
         Walk<CG, SWAP> walk(g, tile_start, row_start, unit, units);
         const Tile t = walk.tile();
-        const int each = run_of(g.width, g.split), ch = thread % 128, channel = t.channel + ch;
-        const int first = int(rank) * each, count = min(each, t.token_end - t.token - first);
-        const float sb = channel < g.N ? __ldg(g.b_scale + t.scale + ch) : 0.0f;
+        const int each = run_of(g.width, g.split), on_lane = thread % 128;
+        const int first = int(rank) * each, count = min(each, columns_of(t) - first);
+        const bool there = on_lane < (SWAP ? g.N - t.channel : t.token_end - t.token);
+        const float own = there ? __ldg(SWAP ? g.b_scale + t.scale + on_lane : g.a_scale + t.token + on_lane) : 0.0f;
         by_out(g.out, [&](auto out) {
-            constexpr int OUT = decltype(out)::value;
+            constexpr int OUT = decltype(out)::value, SIZE = OUT == DTYPE_F32 ? 4 : 2;
             #pragma unroll 2
             for (int group = thread / 128; group * 4 < count; group += 2) {
-                int4 sum = room[group * 128 + ch];
+                int4 sum = room[group * 128 + on_lane];
                 for (int s = 1; s < g.split; ++s) {
-                    const int4 v = room[(s * (each / 4) + group) * 128 + ch];
+                    const int4 v = room[(s * (each / 4) + group) * 128 + on_lane];
                     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
                 }
-                const int part[4] = {sum.x, sum.y, sum.z, sum.w}, token = t.token + first + group * 4;
+                const int part[4] = {sum.x, sum.y, sum.z, sum.w}, column = first + group * 4;
                 float f[4];
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = scaled(uint32_t(part[i]), token_scale[first + group * 4 + i], sb);
-                store_column<OUT>(g.c + size_t(token) * g.N * (OUT == DTYPE_F32 ? 4 : 2), g.N, channel, channel < g.N, f, count - group * 4, thread & 31);
+                for (int i = 0; i < 4; ++i)
+                    f[i] = SWAP ? scaled(uint32_t(part[i]), column_scale[column + i], own) : scaled(uint32_t(part[i]), own, column_scale[column + i]);
+                if constexpr (SWAP) {
+                    const int channel = t.channel + on_lane;
+                    store_column<OUT>(g.c + size_t(t.token + column) * g.N * SIZE, g.N, channel, there, f, count - group * 4, thread & 31);
+                } else if (there) {                              // four channels of one token (their number is a multiple of four)
+                    uint8_t* dst = g.c + (size_t(t.token + on_lane) * g.N + t.channel + column) * SIZE;
+                    if constexpr (OUT == DTYPE_F32) *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+                    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<OUT>(f[0], f[1]), pack_pair<OUT>(f[2], f[3]));
+                }
             }
         });
     }
@@ -481,7 +492,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     int* tile_start = reinterpret_cast<int*>(behind + CONTROL_BYTES);        // grouped: [experts + 1]
     int* row_start = tile_start + g.experts + 1;                             // grouped: first row and first row behind, [experts][2]
     int4* room = reinterpret_cast<int4*>(tile_start);                        // split: partial sums
-    float* token_scale = reinterpret_cast<float*>(behind + CONTROL_BYTES) - 256;     // split: at the control block's end
+    float* column_scale = reinterpret_cast<float*>(behind + CONTROL_BYTES) - 256;     // split: at the control block's end
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool cluster = CG == 2 || g.split > 1;
     const uint32_t rank = cluster ? cluster_ctarank() : 0u;
@@ -565,7 +576,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     } else if (warp == 4) {
         if (CG == 1 || rank == 0) roles.issue(tmem, acc_stride, lane);
     } else if (g.split > 1) {
-        roles.send(tmem, smem_u32(room), token_scale, warp & 3, half, lane);
+        roles.send(tmem, smem_u32(room), column_scale, warp & 3, half, lane);
     } else {
         roles.drain(tmem, acc_stride, warp & 3, half, lane);
         if (g.offsets && g.zero_rest) {
@@ -585,7 +596,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     tc_fence_before_sync();
     if (cluster) { cluster_arrive(); cluster_wait(); }
     __syncthreads();
-    if (g.split > 1 && drains && !ctrl->wait.abort) roles.finish(room, token_scale, thread);
+    if (g.split > 1 && drains && !ctrl->wait.abort) roles.finish(room, column_scale, thread);
     if (warp == 4) {
         tc_fence_after_sync();
         tmem_dealloc<CG>(tmem, columns);
@@ -631,7 +642,7 @@ int resident(int device, int members) {
 }
 int resident(const Int8Tiles& t, int device) {
     if (t.pair) return t.swap ? resident<2, true>(device, 2) : resident<2, false>(device, 2);
-    return t.swap ? resident<1, true>(device, t.split) : resident<1, false>(device, 1);
+    return t.swap ? resident<1, true>(device, t.split) : resident<1, false>(device, t.split);
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
@@ -646,8 +657,9 @@ size_t table_bytes(const Int8Tiles& t, int experts) {
 // Estimated time in ns of a dense product on tiles t: launch and first data, the K loop, the exposed end of the last tile.
 // The loop takes, per 128 values of K and wave, what the tensor cores need for a column (1.03 ns), what an SM takes in of
 // both operands (130 bytes a ns) or what the instructions of a step cost, whichever is longest, and at least as long as
-// the weights need to arrive. The constants are a fit to 1949 timings (M = 1..4096, 11 shapes of N = 520..28672, K =
-// 1024..16384, all forms): what they pick is 0.2 % slower than the fastest on the mean, 4.6 % at worst.
+// both operands need to arrive. The constants are a fit to 1949 timings (M = 1..4096, 11 shapes of N = 520..28672, K =
+// 1024..16384, all forms but the split one with tokens on the M side): what they pick is 0.2 % slower than the fastest on
+// the mean, 4.6 % at worst. The split form with tokens on the M side takes what the other split form takes.
 float estimate(const Int8Tiles& t, int rows, int n, int k, int fit, int sms) {
     const int x = t.pair ? 256 : 128, x_rows = t.swap ? n : rows, y_rows = t.swap ? rows : n;
     const long long tiles = (long long)((x_rows + x - 1) / x) * ((y_rows + t.width - 1) / t.width), waves = (tiles + fit - 1) / fit;
@@ -655,7 +667,7 @@ float estimate(const Int8Tiles& t, int rows, int n, int k, int fit, int sms) {
     const int taken = t.pair ? 128 + t.width / 2 : t.swap ? 128 + std::min(t.width, few) : std::min(128, few) + t.width;
     const float step = std::max({1.03f * float(t.width), float(taken * ROW_BYTES) / 130.0f, t.pair || t.swap ? 190.0f : 170.0f});
     const int ctas = int(std::min((long long)(sms), tiles * (t.pair ? 2 : t.split)));
-    const float hbm = float(n) * float(k) / std::min(7930.0f, 92.5f * float(ctas));
+    const float hbm = (float(n) + float(rows)) * float(k) / std::min(7930.0f, 92.5f * float(ctas));
     const float loop = float(waves) * float((boxes + t.split - 1) / t.split) * step;
     return 3100.0f + (t.pair ? 1100.0f : 0.0f) + std::max(hbm, loop) + 16.0f * float(t.width) + 1570.0f * float(waves - 1) +
            (t.split > 1 ? 1070.0f + 12.0f * float(t.width) : 0.0f);
@@ -684,17 +696,23 @@ Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device) {
             const float ns = estimate(t, rows, n, k, fit, sms);
             if (best.width == 0 || ns < best_ns) { best = t; best_ns = ns; }
         };
-        if (rows <= 128) {
-            const int steps = (k + SUBS<1> * ROW_BYTES - 1) / (SUBS<1> * ROW_BYTES);
+        const int steps = (k + SUBS<1> * ROW_BYTES - 1) / (SUBS<1> * ROW_BYTES);
+        if (rows <= 128)
             for (int split = 1; split <= 8 && (split == 1 || steps / split >= 2); split *= 2) consider(0, 1, round_up(rows, 16), split);
-            // as wide as it takes for one, two or three tiles per SM
+        if (rows > 128)
+            for (int width = 32; width <= 256; width += 32) consider(1, 0, width, 1);
+        // Single CTAs with tokens on the M side: as wide as it takes for one, two or three tiles per SM, for few tokens; and,
+        // where all tiles are resident at once, a cluster to a tile.
+        const int high = (rows + 127) / 128;
+        if (high == 1)
             for (int waves = 1, last = 0; waves <= 3; ++waves) {
                 const int width = std::min(256, round_up((n + waves * sms - 1) / (waves * sms), 16));
                 if (width != last) consider(0, 0, width, 1);
                 last = width;
             }
-        } else {
-            for (int width = 32; width <= 256; width += 32) consider(1, 0, width, 1);
+        for (int split = 2; split <= 8 && steps / split >= 4 && high * split <= sms; split *= 2) {
+            const int across = std::max(1, resident<1, false>(device, split) / high), width = round_up((n + across - 1) / across, 16);
+            if (width <= 128) consider(0, 0, width, split);
         }
     }
     best.subs = subs_for(best);

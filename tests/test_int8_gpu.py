@@ -139,7 +139,7 @@ def assert_product(c, want):
 SIZES = ((1, 8, 16), (1, 128, 128), (2, 136, 4096), (7, 264, 144), (16, 1024, 4096), (17, 512, 2064), (64, 200, 2048),
          (96, 2048, 8192), (128, 1000, 512), (130, 384, 272), (200, 136, 1040), (256, 512, 1024), (257, 520, 400),
          (300, 1000, 992), (513, 2056, 640), (700, 264, 3184), (1024, 1024, 1024),
-         (48, 1000, 4096), (65, 1024, 8192), (9, 8192, 4096), (5, 18944, 1024), (128, 28672, 272), (300, 8200, 528))
+         (48, 1000, 4096), (65, 1024, 8192), (2885, 64, 4112), (300, 520, 8192), (130, 2048, 16384), (640, 136, 5008), (9, 8192, 4096), (5, 18944, 1024), (128, 28672, 272), (300, 8200, 528))
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -159,7 +159,8 @@ def test_every_kernel_is_reached(g):
     tiles = [g.int8_tiles(*size) for size in SIZES]
     assert {(t["pair"], t["swap"]) for t in tiles} == {(1, 0), (0, 0), (0, 1)}
     assert {t["split"] for t in tiles if t["swap"]} == {1, 2, 4, 8}
-    assert {t["width"] for t in tiles if t["swap"]} >= {16, 32, 96} and {t["width"] for t in tiles if t["pair"]} >= {32, 64, 96}
+    assert {t["split"] for t in tiles if not t["swap"] and not t["pair"]} >= {1, 2, 4, 8}
+    assert {t["width"] for t in tiles if t["swap"]} >= {16, 32, 48} and len({t["width"] for t in tiles if t["pair"]}) >= 3
 
 
 @pytest.mark.parametrize("m", (1, 300))
