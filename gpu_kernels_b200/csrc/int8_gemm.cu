@@ -21,7 +21,7 @@
 //     one width for all, 256 experts of unequal popularity took 1143 us instead of 891 in a loop (4096 tokens of six
 //     routes). A tile that reaches into the next expert's rows (or channels) computes them with the wrong weights and does
 //     not store them.
-// Measured: 8192 cubed 326 us (3.37 POPS, twice the rate cuBLAS reaches in bf16; 359 under the power cap); 1 x 8192 x 8192
+// Measured: 8192 cubed 314 us (3.50 POPS, twice the rate cuBLAS reaches in bf16; 359 under the power cap); 1 x 8192 x 8192
 // 15.2 us (4.4 TB/s), 1 x 28672 x 8192 40.4 us (5.8 TB/s), 128 x 28672 x 8192 44 us; 256 experts of 4096 x 4096 with 64
 // tokens of six routes each 470 us (7.1 TB/s).
 #include "operators_internal.h"
@@ -340,30 +340,55 @@ struct Roles {
         }
     };
     // 32 accumulator columns of one lane. Tokens on the lanes: 32 channels of one row of C, in 32-byte stores where every
-    // row starts on a 32-byte boundary (16-byte ones write each sector of C in two halves).
+    // row starts on a 32-byte boundary. 16-byte stores of a lane's own row would write each sector of C in two halves:
+    // where rows start between boundaries (N an odd multiple of 8, 16-bit values) four lanes exchange their 16-byte pieces,
+    // so that each of four stores writes 64 bytes in a row of eight rows (4820 x 24408 x 320: 147 us without).
     template <int OUT>
-    __device__ __forceinline__ void store_row(const uint32_t (&v)[32], const Tile& t, int token, float own, float across, int column, int wide) const {
-        constexpr int SIZE = OUT == DTYPE_F32 ? 4 : 2, PER = 32 / SIZE;          // values in 32 bytes
+    __device__ __forceinline__ void store_row(const uint32_t (&v)[32], const Tile& t, int token, float own, float across, int column, int wide, int lane) const {
+        constexpr int SIZE = OUT == DTYPE_F32 ? 4 : 2, WORDS = 8 * SIZE;
         uint8_t* row = g.c + (size_t(token) * g.N + t.channel + column) * SIZE;
-        const int count = token < t.token_end ? wide - column : 0;               // a multiple of 8, of 16 with rows_32 and 16-bit values
+        const int left = wide - column, count = token < t.token_end ? left : 0;  // multiples of 8, of 16 with rows_32 and 16-bit values
+        uint32_t w[WORDS];
         #pragma unroll
-        for (int q = 0; q < 32 / PER; ++q) {
-            uint32_t w[8];
+        for (int i = 0; i < WORDS; ++i) {
+            const int at = i * (4 / SIZE);
+            const float f = scaled(v[at], own, __shfl_sync(0xFFFFFFFFu, across, at));
+            if constexpr (OUT == DTYPE_F32) w[i] = __float_as_uint(f);
+            else w[i] = pack_pair<OUT>(f, scaled(v[at + 1], own, __shfl_sync(0xFFFFFFFFu, across, at + 1)));
+        }
+        if (g.rows_32) {
             #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = q * PER + i * (4 / SIZE);
-                const float f = scaled(v[at], own, __shfl_sync(0xFFFFFFFFu, across, at));
-                if constexpr (OUT == DTYPE_F32) w[i] = __float_as_uint(f);
-                else w[i] = pack_pair<OUT>(f, scaled(v[at + 1], own, __shfl_sync(0xFFFFFFFFu, across, at + 1)));
-            }
-            uint8_t* dst = row + q * 32;
-            if (g.rows_32) {
-                if (q * PER < count)
+            for (int q = 0; q < WORDS; q += 8)
+                if (q * (4 / SIZE) < count)
                     asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                                 :: "l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-            } else {
-                if (q * PER < count) reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                if (q * PER + PER / 2 < count) reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                                 :: "l"(row + q * 4), "r"(w[q]), "r"(w[q + 1]), "r"(w[q + 2]), "r"(w[q + 3]), "r"(w[q + 4]), "r"(w[q + 5]),
+                                    "r"(w[q + 6]), "r"(w[q + 7]) : "memory");
+        } else if constexpr (OUT == DTYPE_F32) {
+            #pragma unroll
+            for (int q = 0; q < WORDS; q += 4)
+                if (q < count) *reinterpret_cast<uint4*>(row + q * 4) = make_uint4(w[q], w[q + 1], w[q + 2], w[q + 3]);
+        } else {
+            const int r = lane & 3;                              // of the four lanes: afterwards piece r of each of their rows
+            #pragma unroll
+            for (int bit = 1; bit < 4; bit *= 2)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i & bit) continue;
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t& low = w[4 * i + j];
+                        uint32_t& high = w[4 * (i | bit) + j];
+                        const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, r & bit ? low : high, bit);
+                        if (r & bit) low = got;
+                        else high = got;
+                    }
+                }
+            uint8_t* dst = row - size_t(r) * g.N * SIZE + r * 16;
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (token - r + k < t.token_end && 8 * r < left)
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                dst += size_t(g.N) * SIZE;
             }
         }
     }
@@ -396,16 +421,18 @@ struct Roles {
             tc_fence_after_sync();
             const uint32_t acc = tmem + b * acc_stride + (uint32_t(quarter * 32) << 16);
             const int wide = SWAP ? t.token_end - t.token : min(g.width, g.N - t.channel);     // the tile's columns
+            // the next chunk is on its way while one is scaled and stored
+            uint32_t v[2][32];
+            if (half * 32 < wide) tmem_ld_32x32(acc + half * 32, v[0]);
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int column = half * 32 + c * 64;
                 if (column >= wide) break;
-                uint32_t v[32];
-                tmem_ld_32x32(acc + column, v);
                 tmem_ld_wait();
+                if (c < 3 && column + 64 < wide) tmem_ld_32x32(acc + column + 64, v[(c + 1) % 2]);
                 by_out(g.out, [&](auto out) {
-                    if constexpr (SWAP) store_columns<decltype(out)::value>(v, t, t.channel + on_lane, scales.own, scales.across[c], column, wide, lane);
-                    else store_row<decltype(out)::value>(v, t, t.token + on_lane, scales.own, scales.across[c], column, wide);
+                    if constexpr (SWAP) store_columns<decltype(out)::value>(v[c % 2], t, t.channel + on_lane, scales.own, scales.across[c], column, wide, lane);
+                    else store_row<decltype(out)::value>(v[c % 2], t, t.token + on_lane, scales.own, scales.across[c], column, wide, lane);
                 });
                 __syncwarp();
             }

@@ -155,6 +155,18 @@ def test_product(g, m, n, k):
         assert out[0].isnan().all() and out[m + 1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("m, n, k, ahead", ((3, 8, 16, 16), (131, 136, 64, 16), (258, 520, 144, 16), (257, 272, 144, 48), (513, 1048, 256, 32)))
+def test_rows_of_c_on_16_byte_boundaries(g, m, n, k, ahead, dtype):
+    a, b, sa, sb = random_codes((m, k), m), random_codes((n, k), n), random_scales((m,), 1), random_scales((n,), 2)
+    guard = ahead // dtype.itemsize
+    memory = torch.full((guard + m * n + 256,), float("nan"), dtype=dtype, device="cuda")
+    out = memory[guard:guard + m * n].view(m, n)
+    g.int8_gemm(a, b, sa, sb, out=out)
+    assert_product(out, exact(a, b, sa, sb))
+    assert memory[:guard].isnan().all() and memory[guard + m * n:].isnan().all()
+
+
 def test_every_kernel_is_reached(g):
     tiles = [g.int8_tiles(*size) for size in SIZES]
     assert {(t["pair"], t["swap"]) for t in tiles} == {(1, 0), (0, 0), (0, 1)}
