@@ -21,7 +21,7 @@
 //     one width for all, 256 experts of unequal popularity took 1143 us instead of 891 in a loop (4096 tokens of six
 //     routes). A tile that reaches into the next expert's rows (or channels) computes them with the wrong weights and does
 //     not store them.
-// Measured: 8192 cubed 314 us (3.50 POPS, twice the rate cuBLAS reaches in bf16; 359 under the power cap); 1 x 8192 x 8192
+// Measured: 8192 cubed 326 us (3.37 POPS, twice the rate cuBLAS reaches in bf16; 359 under the power cap); 1 x 8192 x 8192
 // 15.2 us (4.4 TB/s), 1 x 28672 x 8192 40.4 us (5.8 TB/s), 128 x 28672 x 8192 44 us; 256 experts of 4096 x 4096 with 64
 // tokens of six routes each 470 us (7.1 TB/s).
 #include "operators_internal.h"
@@ -340,34 +340,43 @@ struct Roles {
         }
     };
     // 32 accumulator columns of one lane. Tokens on the lanes: 32 channels of one row of C, in 32-byte stores where every
-    // row starts on a 32-byte boundary. 16-byte stores of a lane's own row would write each sector of C in two halves:
-    // where rows start between boundaries (N an odd multiple of 8, 16-bit values) four lanes exchange their 16-byte pieces,
-    // so that each of four stores writes 64 bytes in a row of eight rows (4820 x 24408 x 320: 147 us without).
+    // row starts on a 32-byte boundary. 16-byte stores of a lane's own row write each sector of C in two halves: where rows
+    // start between boundaries (N an odd multiple of 8, 16-bit values) four lanes of a pair's kernel, whose many tokens may
+    // make C the bound, exchange their 16-byte pieces, so that each of four stores writes 64 bytes of eight rows
+    // (4820 x 24408 x 320: 84 us, without 146; 3000 x 8200 x 1024: 24.7 and 28.2).
     template <int OUT>
     __device__ __forceinline__ void store_row(const uint32_t (&v)[32], const Tile& t, int token, float own, float across, int column, int wide, int lane) const {
         constexpr int SIZE = OUT == DTYPE_F32 ? 4 : 2, WORDS = 8 * SIZE;
         uint8_t* row = g.c + (size_t(token) * g.N + t.channel + column) * SIZE;
         const int left = wide - column, count = token < t.token_end ? left : 0;  // multiples of 8, of 16 with rows_32 and 16-bit values
-        uint32_t w[WORDS];
-        #pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            const int at = i * (4 / SIZE);
-            const float f = scaled(v[at], own, __shfl_sync(0xFFFFFFFFu, across, at));
-            if constexpr (OUT == DTYPE_F32) w[i] = __float_as_uint(f);
-            else w[i] = pack_pair<OUT>(f, scaled(v[at + 1], own, __shfl_sync(0xFFFFFFFFu, across, at + 1)));
-        }
+        auto words = [&](uint32_t* w, int first, int n) {       // of the row's 32 values, as stored
+            #pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const int at = (first + i) * (4 / SIZE);
+                const float f = scaled(v[at], own, __shfl_sync(0xFFFFFFFFu, across, at));
+                if constexpr (OUT == DTYPE_F32) w[i] = __float_as_uint(f);
+                else w[i] = pack_pair<OUT>(f, scaled(v[at + 1], own, __shfl_sync(0xFFFFFFFFu, across, at + 1)));
+            }
+        };
         if (g.rows_32) {
             #pragma unroll
-            for (int q = 0; q < WORDS; q += 8)
+            for (int q = 0; q < WORDS; q += 8) {
+                uint32_t w[8];
+                words(w, q, 8);
                 if (q * (4 / SIZE) < count)
                     asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                                 :: "l"(row + q * 4), "r"(w[q]), "r"(w[q + 1]), "r"(w[q + 2]), "r"(w[q + 3]), "r"(w[q + 4]), "r"(w[q + 5]),
-                                    "r"(w[q + 6]), "r"(w[q + 7]) : "memory");
-        } else if constexpr (OUT == DTYPE_F32) {
+                                 :: "l"(row + q * 4), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+            }
+        } else if constexpr (OUT == DTYPE_F32 || CG == 1) {
             #pragma unroll
-            for (int q = 0; q < WORDS; q += 4)
-                if (q < count) *reinterpret_cast<uint4*>(row + q * 4) = make_uint4(w[q], w[q + 1], w[q + 2], w[q + 3]);
+            for (int q = 0; q < WORDS; q += 4) {
+                uint32_t w[4];
+                words(w, q, 4);
+                if (q * (4 / SIZE) < count) *reinterpret_cast<uint4*>(row + q * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         } else {
+            uint32_t w[WORDS];
+            words(w, 0, WORDS);
             const int r = lane & 3;                              // of the four lanes: afterwards piece r of each of their rows
             #pragma unroll
             for (int bit = 1; bit < 4; bit *= 2)
@@ -421,18 +430,16 @@ struct Roles {
             tc_fence_after_sync();
             const uint32_t acc = tmem + b * acc_stride + (uint32_t(quarter * 32) << 16);
             const int wide = SWAP ? t.token_end - t.token : min(g.width, g.N - t.channel);     // the tile's columns
-            // the next chunk is on its way while one is scaled and stored
-            uint32_t v[2][32];
-            if (half * 32 < wide) tmem_ld_32x32(acc + half * 32, v[0]);
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int column = half * 32 + c * 64;
                 if (column >= wide) break;
+                uint32_t v[32];
+                tmem_ld_32x32(acc + column, v);
                 tmem_ld_wait();
-                if (c < 3 && column + 64 < wide) tmem_ld_32x32(acc + column + 64, v[(c + 1) % 2]);
                 by_out(g.out, [&](auto out) {
-                    if constexpr (SWAP) store_columns<decltype(out)::value>(v[c % 2], t, t.channel + on_lane, scales.own, scales.across[c], column, wide, lane);
-                    else store_row<decltype(out)::value>(v[c % 2], t, t.token + on_lane, scales.own, scales.across[c], column, wide, lane);
+                    if constexpr (SWAP) store_columns<decltype(out)::value>(v, t, t.channel + on_lane, scales.own, scales.across[c], column, wide, lane);
+                    else store_row<decltype(out)::value>(v, t, t.token + on_lane, scales.own, scales.across[c], column, wide, lane);
                 });
                 __syncwarp();
             }
