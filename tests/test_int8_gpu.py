@@ -188,7 +188,7 @@ def test_longest_sum(g, m):
 
 
 @pytest.mark.parametrize("dtype,out", ((BF16, None), (F16, F32), (F32, BF16)))
-@pytest.mark.parametrize("m,n,k", ((1, 4096, 4096), (5, 72, 48), (33, 1024, 8192), (300, 512, 1024), (1000, 1032, 2000)))
+@pytest.mark.parametrize("m,n,k", ((1, 4096, 4096), (5, 72, 48), (33, 1024, 8192), (300, 512, 1024), (1000, 1032, 2000), (400, 1536, 8208), (2000, 72, 4112)))
 def test_linear_is_quantise_then_product(g, m, n, k, dtype, out):
     x = normal((m, k), dtype, m)
     w, ws = g.quantize_int8(normal((n, k), BF16, n, 0.02))
