@@ -174,8 +174,10 @@ __device__ __forceinline__ float scaled(uint32_t sum, float token, float channel
 __host__ __device__ __forceinline__ int run_of(int width, int split) { return (width + 4 * split - 1) / (4 * split) * 4; }
 
 // Boxes of 128 K values per operand and ring stage, at most (Args::subs). Two where tiles are narrow: a step's instructions
-// (one wait, one request per box, the MMAs, one commit) are then what bounds it. Wide tiles keep the finer ring.
-template <int CG> constexpr int SUBS = CG == 1 ? 2 : 1;
+// (waits, commits, requests) then serve twice the bytes (pairs: 2048 x 1024 x 8192, width 128, 19.4 -> 17.4 us; width 192
+// 20.5 either way). Wide tiles keep the finer ring, and roles of their own: in the code for two 1536 x 2048 x 8192 took 25.2
+// us instead of 20.5.
+constexpr int SUBS = 2;
 
 template <int CG, bool SWAP>
 struct Roles {
@@ -223,16 +225,18 @@ struct Roles {
         }
     };
     // Boxes of a ring step that lie in K: those beyond would be zeros.
-    __device__ __forceinline__ int boxes(int ks) const { return SUBS<CG> == 1 ? 1 : min(g.subs, g.kboxes - ks * g.subs); }
+    template <int S>
+    __device__ __forceinline__ int boxes(int ks) const { return S == 1 ? 1 : min(g.subs, g.kboxes - ks * g.subs); }
     // One operand's part of ring stage `stage`; x_side: the M side's.
+    template <int S>
     __device__ __forceinline__ void request(const CUtensorMap* map, bool x_side, const Cursor& c, int stage) const {
         constexpr int MOST = SWAP ? 4 : 1;                      // boxes of 32 rows in 128 (a pair: 256 / 2)
         const uint32_t dst = smem + stage * stage_bytes + (x_side ? 0u : uint32_t(g.subs) * 128u * ROW_BYTES);
         const uint32_t full = smem_u32(&ctrl->full[stage]), bar = CG == 2 ? map_to_cta(full, 0) : full;
         const uint32_t pitch = (x_side ? 128u : uint32_t(g.width / CG)) * ROW_BYTES, part = uint32_t(g.y_box) * ROW_BYTES;
-        const int n = boxes(c.ks);
+        const int n = boxes<S>(c.ks);
         #pragma unroll
-        for (int s = 0; s < SUBS<CG>; ++s) {
+        for (int s = 0; s < S; ++s) {
             if (s >= n) break;
             const int k = (c.ks * g.subs + s) * ROW_BYTES;
             #pragma unroll
@@ -243,6 +247,7 @@ struct Roles {
             }
         }
     }
+    template <int S>
     __device__ void produce(const CUtensorMap* mapX, const CUtensorMap* mapY, int lane) const {
         const CUtensorMap* weights = SWAP ? mapX : mapY;
         const CUtensorMap* tokens = SWAP ? mapY : mapX;
@@ -255,12 +260,12 @@ struct Roles {
             int lead = 0;
             for (; lead < g.stages && ahead.valid(); ++lead, ahead.next())
                 if (elect_one()) {
-                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[lead]), ahead.bytes * boxes(ahead.ks));
-                    request(weights, SWAP, ahead, lead);
+                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[lead]), ahead.bytes * boxes<S>(ahead.ks));
+                    request<S>(weights, SWAP, ahead, lead);
                 }
             grid_dependency_wait();
             for (int i = 0; i < lead; ++i, cursor.next())
-                if (elect_one()) request(tokens, !SWAP, cursor, i);
+                if (elect_one()) request<S>(tokens, !SWAP, cursor, i);
             if (lead == g.stages) phase = 1;
             else stage = lead;
         }
@@ -268,15 +273,16 @@ struct Roles {
             const bool ok = wait(&ctrl->empty[stage], phase ^ 1u, lane == 0 ? STATUS_TIMEOUT_PRODUCER : 0u, 0x50000000u | (stage << 16) | cursor.ks);
             if (!__all_sync(0xFFFFFFFFu, ok)) return;
             if (elect_one()) {
-                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[stage]), cursor.bytes * boxes(cursor.ks));
-                request(weights, SWAP, cursor, stage);
-                request(tokens, !SWAP, cursor, stage);
+                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(smem_u32(&ctrl->full[stage]), cursor.bytes * boxes<S>(cursor.ks));
+                request<S>(weights, SWAP, cursor, stage);
+                request<S>(tokens, !SWAP, cursor, stage);
             }
             if (++stage == g.stages) { stage = 0; phase ^= 1u; }
         }
     }
 
     // ---- warp 4 (of the pair's first CTA) -------------------------------------------------------------------------
+    template <int S>
     __device__ void issue(uint32_t tmem, uint32_t acc_stride, int lane) const {
         // Operand descriptors: rows of 128 bytes under the 128-byte swizzle, 8-row groups 1024 bytes apart, version 1.
         constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -303,9 +309,9 @@ struct Roles {
                 const bool probe = mbar_test_wait(smem_u32(&ctrl->full[next_stage]), next_phase);
                 const uint32_t lo = ring_lo + uint32_t(stage) * (stage_bytes >> 4);
                 if (elect_one()) {
-                    const int n = boxes(ks);
+                    const int n = boxes<S>(ks);
                     #pragma unroll
-                    for (int s = 0; s < SUBS<CG>; ++s) {
+                    for (int s = 0; s < S; ++s) {
                         if (s >= n) break;
                         const uint32_t x = lo + (s * 128 * ROW_BYTES >> 4), y = lo + uint32_t(g.subs) * (128 * ROW_BYTES >> 4) + s * y_pitch;
                         #pragma unroll
@@ -605,10 +611,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     const bool drains = warp < 4 || warp >= 6;
     const int half = warp < 4 ? 0 : 1, thread = (half * 4 + (warp & 3)) * 32 + lane;
     if (warp == 5) {
-        roles.produce(&mapX, &mapY, lane);
+        if ((CG == 1 || !SWAP) && g.subs > 1) roles.template produce<SUBS>(&mapX, &mapY, lane);
+        else roles.template produce<1>(&mapX, &mapY, lane);
         if (g.early) grid_launch_dependents();                   // (its wait lies behind it)
     } else if (warp == 4) {
-        if (CG == 1 || rank == 0) roles.issue(tmem, acc_stride, lane);
+        if (CG == 1 || rank == 0) {
+            if ((CG == 1 || !SWAP) && g.subs > 1) roles.template issue<SUBS>(tmem, acc_stride, lane);
+            else roles.template issue<1>(tmem, acc_stride, lane);
+        }
     } else if (g.split > 1) {
         roles.send(tmem, smem_u32(room), column_scale, warp & 3, half, lane);
     } else {
@@ -682,7 +692,7 @@ int resident(const Int8Tiles& t, int device) {
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
 size_t stage_size(const Int8Tiles& t) { return size_t(t.subs) * (128 + t.width / (t.pair ? 2 : 1)) * ROW_BYTES; }
-int subs_for(const Int8Tiles& t) { return t.pair || t.width > WIDE_FROM ? 1 : SUBS<1>; }
+int subs_for(const Int8Tiles& t) { return t.width > (t.pair ? 160 : WIDE_FROM) ? 1 : SUBS; }
 
 size_t table_bytes(const Int8Tiles& t, int experts) {
     return experts ? size_t(3 * experts + 1) * sizeof(int) : t.split > 1 ? size_t(t.split) * run_of(t.width, t.split) * 128 * sizeof(int) : 0;
@@ -730,7 +740,7 @@ Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device) {
             const float ns = estimate(t, rows, n, k, fit, sms);
             if (best.width == 0 || ns < best_ns) { best = t; best_ns = ns; }
         };
-        const int steps = (k + SUBS<1> * ROW_BYTES - 1) / (SUBS<1> * ROW_BYTES);
+        const int steps = (k + SUBS * ROW_BYTES - 1) / (SUBS * ROW_BYTES);
         if (rows <= 128)
             for (int split = 1; split <= 8 && (split == 1 || steps / split >= 2); split *= 2) consider(0, 1, round_up(rows, 16), split);
         if (rows > 128)
