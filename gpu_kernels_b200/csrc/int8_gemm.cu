@@ -699,22 +699,22 @@ size_t table_bytes(const Int8Tiles& t, int experts) {
 }
 
 // Estimated time in ns of a dense product on tiles t: launch and first data, the K loop, the exposed end of the last tile.
-// The loop takes, per 128 values of K and wave, what the tensor cores need for a column (1.03 ns), what an SM takes in of
-// both operands (130 bytes a ns) or what the instructions of a step cost, whichever is longest, and at least as long as
-// both operands need to arrive. The constants are a fit to 1949 timings (M = 1..4096, 11 shapes of N = 520..28672, K =
-// 1024..16384, all forms but the split one with tokens on the M side): what they pick is 0.2 % slower than the fastest on
-// the mean, 4.6 % at worst. The split form with tokens on the M side takes what the other split form takes.
+// The loop takes, per 128 values of K and wave, what the tensor cores need for a column (1.04 ns), what an SM takes in of
+// both operands (139 bytes a ns) or what the instructions of a step cost (164 ns in a stage of two boxes, 211 in one of
+// one), whichever is longest, and at least as long as both operands need to arrive. The constants are a fit to 2896 timings
+// (M = 1..4096, 13 shapes of N = 512..28672, K = 2000..16384, all forms): what they pick is 0.3 % slower than the fastest on
+// the mean, 11 % at worst (192 x 1032 x 2000).
 float estimate(const Int8Tiles& t, int rows, int n, int k, int fit, int sms) {
     const int x = t.pair ? 256 : 128, x_rows = t.swap ? n : rows, y_rows = t.swap ? rows : n;
     const long long tiles = (long long)((x_rows + x - 1) / x) * ((y_rows + t.width - 1) / t.width), waves = (tiles + fit - 1) / fit;
     const int few = round_up(rows, 8), boxes = (k + ROW_BYTES - 1) / ROW_BYTES;
     const int taken = t.pair ? 128 + t.width / 2 : t.swap ? 128 + std::min(t.width, few) : std::min(128, few) + t.width;
-    const float step = std::max({1.03f * float(t.width), float(taken * ROW_BYTES) / 130.0f, t.pair || t.swap ? 190.0f : 170.0f});
+    const float step = std::max({1.04f * float(t.width), float(taken * ROW_BYTES) / 139.0f, subs_for(t) > 1 ? 164.0f : 211.0f});
     const int ctas = int(std::min((long long)(sms), tiles * (t.pair ? 2 : t.split)));
-    const float hbm = (float(n) + float(rows)) * float(k) / std::min(7930.0f, 92.5f * float(ctas));
+    const float hbm = (float(n) + float(rows)) * float(k) / std::min(8120.0f, 91.6f * float(ctas));
     const float loop = float(waves) * float((boxes + t.split - 1) / t.split) * step;
-    return 3100.0f + (t.pair ? 1100.0f : 0.0f) + std::max(hbm, loop) + 16.0f * float(t.width) + 1570.0f * float(waves - 1) +
-           (t.split > 1 ? 1070.0f + 12.0f * float(t.width) : 0.0f);
+    return 3740.0f + (t.pair ? 700.0f : 0.0f) + std::max(hbm, loop) + 14.3f * float(t.width) + 1600.0f * float(waves - 1) +
+           (t.split > 1 ? 1070.0f + 14.8f * float(t.width) : 0.0f);
 }
 
 }  // namespace
@@ -748,9 +748,9 @@ Int8Tiles int8_tiles(int rows, int n, int k, int experts, int device) {
         // Single CTAs with tokens on the M side: as wide as it takes for one, two or three tiles per SM, for few tokens; and,
         // where all tiles are resident at once, a cluster to a tile.
         const int high = (rows + 127) / 128;
-        if (high == 1)
+        if (high <= 2)
             for (int waves = 1, last = 0; waves <= 3; ++waves) {
-                const int width = std::min(256, round_up((n + waves * sms - 1) / (waves * sms), 16));
+                const int across = waves * sms / high, width = std::min(256, round_up((n + across - 1) / across, 16));
                 if (width != last) consider(0, 0, width, 1);
                 last = width;
             }

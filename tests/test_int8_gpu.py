@@ -139,7 +139,7 @@ def assert_product(c, want):
 SIZES = ((1, 8, 16), (1, 128, 128), (2, 136, 4096), (7, 264, 144), (16, 1024, 4096), (17, 512, 2064), (64, 200, 2048),
          (96, 2048, 8192), (128, 1000, 512), (130, 384, 272), (200, 136, 1040), (256, 512, 1024), (257, 520, 400),
          (300, 1000, 992), (513, 2056, 640), (700, 264, 3184), (1024, 1024, 1024),
-         (48, 1000, 4096), (65, 1024, 8192), (2885, 64, 4112), (300, 520, 8192), (130, 2048, 16384), (640, 136, 5008), (9, 8192, 4096), (5, 18944, 1024), (128, 28672, 272), (300, 8200, 528))
+         (48, 1000, 4096), (65, 1024, 8192), (2885, 64, 4112), (300, 520, 8192), (128, 520, 16384), (130, 2048, 16384), (640, 136, 5008), (9, 8192, 4096), (5, 18944, 1024), (128, 28672, 272), (300, 8200, 528))
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
