@@ -6,8 +6,9 @@
 // or an infinity has scale NaN and codes 0: what is computed from it is NaN, not a number that looks sound.
 //
 // HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes (8192 x 8192 bf16
-// 31.6 us, 6.4 TB/s; FP32 52 us; 8192 x 8191 bf16 34.7). Threads take 16
-// values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
+// 31.6 us, 6.4 TB/s; FP32 52 us; 8192 x 8191 bf16 34.7). A row is a
+// warp's, or that of a block of as many warps as hold it (with blocks of 256 or 512 threads 4836 x 8784 FP32 took 64 us
+// instead of 38). Threads take 16 values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
 // and stores are aligned whatever K is; what a row has in front of its first whole group and behind its last one (up to 15
 // values each) is taken by 32 threads, one value each.
 #include "operators_internal.h"
@@ -112,16 +113,15 @@ struct Group {                                                  // 16 values as 
     }
 };
 
-// TPR: threads per row, NV: groups of 16 that each of them holds in registers; what a row has beyond TPR * NV groups is read
-// twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
+// TPR: threads per row, 32 (a warp) or up to that many (a block of as many as it takes); NV: groups of 16 that each of them
+// holds in registers; what a row has beyond those is read twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
 template <typename T, int TPR, int NV, bool ROUTED, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, long long rows, int K,
                      const int* __restrict__ position, const int* __restrict__ live, int topk) {
     ptx::chain_point();
-    constexpr int THREADS = TPR < 256 ? 256 : TPR, ROWS = THREADS / TPR;
-    const int t = threadIdx.x % TPR;
-    const long long row = (long long)(blockIdx.x) * ROWS + threadIdx.x / TPR;
+    const int tpr = TPR == 32 ? 32 : int(blockDim.x), t = TPR == 32 ? threadIdx.x % 32 : threadIdx.x;
+    const long long row = TPR == 32 ? (long long)(blockIdx.x) * 8 + threadIdx.x / 32 : blockIdx.x;
     if (TPR == 32 && row >= rows) return;                       // (a warp's row; otherwise the grid has one block per row)
     const size_t begin = size_t(row) * K, end = begin + K;
     const size_t whole_from = WHOLE ? begin : min(end, (begin + 15) / 16 * 16), whole_to = WHOLE ? end : max(whole_from, end / 16 * 16);
@@ -134,26 +134,28 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
         if constexpr (sizeof(T) == 2) single_bits = __ldg(reinterpret_cast<const unsigned short*>(x) + single);
         else single_bits = __ldg(reinterpret_cast<const uint32_t*>(x) + single);
     }
+    // A warp holds 32 NV groups in a row: its loads and stores differ by constants.
+    const size_t first = g0 + t / 32 * (32 * NV) + t % 32;
     Group<T> held[NV];
     uint32_t top = single_bits & (sizeof(T) == 2 ? 0x7FFFu : 0x7FFFFFFFu);
     #pragma unroll
     for (int j = 0; j < NV; ++j)
-        if (g0 + t + j * TPR < g1) held[j].load(x, g0 + t + j * TPR);
-    for (size_t group = g0 + t + NV * TPR; !WHOLE && group < g1; group += TPR) {
+        if (first + j * 32 < g1) held[j].load(x, first + j * 32);
+    for (size_t group = g0 + t + NV * tpr; !WHOLE && group < g1; group += tpr) {
         Group<T> v;
         v.load(x, group);
         top = v.magnitude(top);
     }
     #pragma unroll
     for (int j = 0; j < NV; ++j)
-        if (g0 + t + j * TPR < g1) top = held[j].magnitude(top);
+        if (first + j * 32 < g1) top = held[j].magnitude(top);
     if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     if constexpr (TPR > 32) {
         __shared__ uint32_t warp_top[TPR / 32];
         if (threadIdx.x % 32 == 0) warp_top[threadIdx.x / 32] = top;
         __syncthreads();
-        const uint32_t mine = threadIdx.x % 32 < TPR / 32 ? warp_top[threadIdx.x % 32] : 0u;
+        const uint32_t mine = threadIdx.x % 32 < blockDim.x / 32 ? warp_top[threadIdx.x % 32] : 0u;
         top = __reduce_max_sync(0xFFFFFFFFu, mine);
     }
     const bool finite = top < Bits<T>::NOT_FINITE;
@@ -176,15 +178,15 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
     if (has_single) codes[single] = finite ? int8_t(code_of<T>(Bits<T>::widen(single_bits), s)) : int8_t(0);
     #pragma unroll
     for (int j = 0; j < NV; ++j)
-        if (g0 + t + j * TPR < g1) emit(held[j], g0 + t + j * TPR);
-    for (size_t group = g0 + t + NV * TPR; !WHOLE && group < g1; group += TPR) {
+        if (first + j * 32 < g1) emit(held[j], first + j * 32);
+    for (size_t group = g0 + t + NV * tpr; !WHOLE && group < g1; group += tpr) {
         Group<T> v;
         v.load(x, group);
         emit(v, group);
     }
     if constexpr (ROUTED) {
         const int end_live = __ldg(live);
-        for (int j = t; j < topk; j += TPR) {
+        for (int j = t; j < topk; j += tpr) {
             const int to = __ldg(position + row * topk + j);
             if (to >= 0 && to < rows * topk) scales[to] = to < end_live ? scale : 0.0f;
         }
@@ -231,27 +233,37 @@ int8_dequantise_kernel(const int8_t* __restrict__ codes, const float* __restrict
 template <typename T, bool ROUTED>
 void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, const int* position, const int* live, int topk,
             cudaStream_t stream) {
-    auto go = [&](auto kernel, int threads, int per_block) {
-        launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads), 0, stream,
+    auto go = [&](auto kernel, int threads) {
+        const int per_block = threads ? 1 : 8;                   // 0: a warp per row
+        launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads ? threads : 256), 0, stream,
                        static_cast<const T*>(x), codes, scales, rows, K, position, live, topk);
     };
     const int groups = K / 16;
-    // A group held is 8 registers of 16-bit values and 16 of FP32: of those no more than two (four left room for two blocks
-    // per SM: 4096 x 16384 FP32 71 us, 8192 x 1024 14 us), but for the longest rows.
+    // As many warps as hold the row, `most` threads at most.
+    auto block = [&](int held, int most) { return std::max(64, std::min(most, (groups + 32 * held - 1) / (32 * held) * 32)); };
+    // A group held is 8 registers of 16-bit values and 16 of FP32: of those no more than two, as blocks of one SM are to be
+    // at different points of their rows. Longer FP32 rows are read again from L2 (K = 28672 1.65 times the time its bytes
+    // take, with four groups 2.2; 14336 in one group to a thread 1.24, in two 1.4; 12288 1.27 and 1.16). 16-bit rows of 4608
+    // to 16384 values take 1.00 to 1.04 times what their bytes take.
     constexpr bool SHORT = sizeof(T) == 2;
     constexpr int MOST = SHORT ? 4 : 2;
-    if (K % 16 || groups > 2048) {
-        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
-        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, 256, 1);
-        else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, 512, 1);
-    } else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 256, 8);
-    else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 256, 8);
-    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 256, 8);
-    else if (groups <= 256) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, 256, 1);
-    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, 256, 1);
-    else if (groups <= 256 * MOST) go(int8_quantise_kernel<T, 256, MOST, ROUTED, true>, 256, 1);
-    else if (groups <= 1024) go(int8_quantise_kernel<T, 512, 2, ROUTED, true>, 512, 1);
-    else go(int8_quantise_kernel<T, 512, 4, ROUTED, true>, 512, 1);
+    if (K % 16 || groups > (SHORT ? 2048 : 1024)) {
+        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 0);
+        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, block(2, 256));
+        else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, block(MOST, 512));
+    } else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 0);
+    else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 0);
+    else if (SHORT && groups <= 96) go(int8_quantise_kernel<T, 32, 3, ROUTED, true>, 0);
+    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 0);
+    else if (groups <= 256 && !SHORT) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, block(1, 256));
+    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, block(2, 256));
+    else if constexpr (SHORT) {
+        if (groups <= 1024) go(int8_quantise_kernel<T, 256, 4, ROUTED, true>, block(4, 256));
+        else go(int8_quantise_kernel<T, 512, 4, ROUTED, true>, block(4, 512));
+    } else {
+        if (groups <= 768) go(int8_quantise_kernel<T, 512, 2, ROUTED, true>, block(2, 512));
+        else go(int8_quantise_kernel<T, 1024, 1, ROUTED, true>, block(1, 1024));
+    }
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
