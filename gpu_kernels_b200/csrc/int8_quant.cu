@@ -113,16 +113,17 @@ struct Group {                                                  // 16 values as 
     }
 };
 
-// TPR: threads per row, 32 (a warp) or up to that many (a block of as many as it takes); NV: groups of 16 that each of them
+// TPR: threads per row, up to 32 (a warp or part of one) or at most that many (a block of as many as it takes); NV: groups of 16 that each of them
 // holds in registers; what a row has beyond those is read twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
 template <typename T, int TPR, int NV, bool ROUTED, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, long long rows, int K,
                      const int* __restrict__ position, const int* __restrict__ live, int topk) {
     ptx::chain_point();
-    const int tpr = TPR == 32 ? 32 : int(blockDim.x), t = TPR == 32 ? threadIdx.x % 32 : threadIdx.x;
-    const long long row = TPR == 32 ? (long long)(blockIdx.x) * 8 + threadIdx.x / 32 : blockIdx.x;
-    if (TPR == 32 && row >= rows) return;                       // (a warp's row; otherwise the grid has one block per row)
+    const int tpr = TPR <= 32 ? TPR : int(blockDim.x), t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
+    long long row = TPR <= 32 ? (long long)(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    if (TPR == 32 && row >= rows) return;
+    if (TPR < 32) row = min(row, rows - 1);                     // (what a warp has behind the last row writes that row's codes again)
     const size_t begin = size_t(row) * K, end = begin + K;
     const size_t whole_from = WHOLE ? begin : min(end, (begin + 15) / 16 * 16), whole_to = WHOLE ? end : max(whole_from, end / 16 * 16);
     const size_t g0 = whole_from / 16, g1 = g0 + (whole_to - whole_from) / 16;
@@ -150,7 +151,12 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
     for (int j = 0; j < NV; ++j)
         if (first + j * 32 < g1) top = held[j].magnitude(top);
     if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if constexpr (TPR < 32) {
+        #pragma unroll
+        for (int d = TPR / 2; d; d /= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    } else {
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+    }
     if constexpr (TPR > 32) {
         __shared__ uint32_t warp_top[TPR / 32];
         if (threadIdx.x % 32 == 0) warp_top[threadIdx.x / 32] = top;
@@ -233,9 +239,8 @@ int8_dequantise_kernel(const int8_t* __restrict__ codes, const float* __restrict
 template <typename T, bool ROUTED>
 void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, const int* position, const int* live, int topk,
             cudaStream_t stream) {
-    auto go = [&](auto kernel, int threads) {
-        const int per_block = threads ? 1 : 8;                   // 0: a warp per row
-        launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads ? threads : 256), 0, stream,
+    auto go = [&](auto kernel, int threads, int per_block = 1) {
+        launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads), 0, stream,
                        static_cast<const T*>(x), codes, scales, rows, K, position, live, topk);
     };
     const int groups = K / 16;
@@ -248,13 +253,16 @@ void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, 
     constexpr bool SHORT = sizeof(T) == 2;
     constexpr int MOST = SHORT ? 4 : 2;
     if (K % 16 || groups > (SHORT ? 2048 : 1024)) {
-        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 0);
+        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
         else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, block(2, 256));
         else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, block(MOST, 512));
-    } else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 0);
-    else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 0);
-    else if (SHORT && groups <= 96) go(int8_quantise_kernel<T, 32, 3, ROUTED, true>, 0);
-    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 0);
+    } else if (groups <= 4) go(int8_quantise_kernel<T, 4, 1, ROUTED, true>, 256, 64);
+    else if (groups <= 8) go(int8_quantise_kernel<T, 8, 1, ROUTED, true>, 256, 32);
+    else if (groups <= 16) go(int8_quantise_kernel<T, 16, 1, ROUTED, true>, 256, 16);
+    else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 256, 8);
+    else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 256, 8);
+    else if (SHORT && groups <= 96) go(int8_quantise_kernel<T, 32, 3, ROUTED, true>, 256, 8);
+    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 256, 8);
     else if (groups <= 256 && !SHORT) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, block(1, 256));
     else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, block(2, 256));
     else if constexpr (SHORT) {

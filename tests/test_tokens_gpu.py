@@ -175,7 +175,9 @@ def test_strides_broadcast_gradients_and_alignment(g):
 
 
 @pytest.mark.parametrize("dtype", (BF16, F16, F32))
-@pytest.mark.parametrize("tokens,topk,experts,k", ((1, 6, 256, 4096), (9, 3, 4, 16), (40, 2, 8, 528), (70, 8, 16, 2064), (2, 2, 4, 33008)))
+@pytest.mark.parametrize("tokens,topk,experts,k", ((1, 6, 256, 4096), (9, 3, 4, 16), (40, 2, 8, 528), (70, 8, 16, 2064), (2, 2, 4, 33008),
+                                                    (11, 2, 8, 1040), (5, 2, 8, 4112), (6, 3, 8, 8784), (4, 2, 8, 14336), (3, 2, 8, 20496), (75, 3, 8, 64), (41, 4, 8, 128),
+                                                    (19, 2, 8, 240)))
 def test_gather_quantised(g, tokens, topk, experts, k, dtype):
     routes = g.sort_routes(choices(tokens, topk, experts, k, 0.2), experts)
     x = normal((tokens, k), dtype, 1)
