@@ -6,11 +6,11 @@
 // or an infinity has scale NaN and codes 0: what is computed from it is NaN, not a number that looks sound.
 //
 // HBM-bound: the row is read once, held in registers while its maximum is taken, and written as codes (8192 x 8192 bf16
-// 31.6 us, 6.4 TB/s; FP32 52 us; 8192 x 8191 bf16 34.7). A row is a
-// warp's, or that of a block of as many warps as hold it (with blocks of 256 or 512 threads 4836 x 8784 FP32 took 64 us
-// instead of 38). Threads take 16 values each, one 16-byte store of codes. The elements of all rows are one flat array cut into groups of 16, so loads
-// and stores are aligned whatever K is; what a row has in front of its first whole group and behind its last one (up to 15
-// values each) is taken by 32 threads, one value each.
+// 31.6 us, 6.4 TB/s; FP32 52 us; 8192 x 8191 bf16 34.7). A row is that of 4 to 32 threads, or of a block of as many warps as
+// hold it (with a warp for each short row 128 values took 4.0 times what their bytes take, now 1.2; with blocks of 256 or
+// 512 threads for each long one 4836 x 8784 FP32 took 64 us, now 38). Threads take 16 values each, one 16-byte store of
+// codes. The elements of all rows are one flat array cut into groups of 16, so loads and stores are aligned whatever K is;
+// what a row has in front of its first whole group and behind its last one (up to 15 values each) is taken one by one.
 #include "operators_internal.h"
 #include "ptx.cuh"
 
@@ -113,8 +113,8 @@ struct Group {                                                  // 16 values as 
     }
 };
 
-// TPR: threads per row, up to 32 (a warp or part of one) or at most that many (a block of as many as it takes); NV: groups of 16 that each of them
-// holds in registers; what a row has beyond those is read twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
+// TPR: threads per row, up to 32 (a warp or part of one) or at most that many (a block of as many as it takes); NV: groups
+// of 16 that each of them holds in registers; what a row has beyond those is read twice, the second time from L2. ROUTED: the row's codes go to `topk` rows of the output instead of its own.
 template <typename T, int TPR, int NV, bool ROUTED, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, long long rows, int K,
@@ -127,21 +127,30 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
     const size_t begin = size_t(row) * K, end = begin + K;
     const size_t whole_from = WHOLE ? begin : min(end, (begin + 15) / 16 * 16), whole_to = WHOLE ? end : max(whole_from, end / 16 * 16);
     const size_t g0 = whole_from / 16, g1 = g0 + (whole_to - whole_from) / 16;
-    // This thread's value outside the whole groups: in front of them for the first sixteen threads, behind for the next.
-    const size_t single = t < 16 ? begin + t : whole_to + (t - 16);
-    const bool has_single = !WHOLE && t < 32 && single < (t < 16 ? whole_from : end);
-    uint32_t single_bits = 0u;
-    if (has_single) {
-        if constexpr (sizeof(T) == 2) single_bits = __ldg(reinterpret_cast<const unsigned short*>(x) + single);
-        else single_bits = __ldg(reinterpret_cast<const uint32_t*>(x) + single);
+    // This thread's values outside the whole groups, 32 places in all: sixteen in front of them and as many behind.
+    constexpr int SINGLES = WHOLE ? 0 : TPR < 32 ? 32 / TPR : 1;
+    size_t place[SINGLES ? SINGLES : 1];
+    bool has_single[SINGLES ? SINGLES : 1];
+    uint32_t single_bits[SINGLES ? SINGLES : 1], top = 0u;
+    #pragma unroll
+    for (int i = 0; i < SINGLES; ++i) {
+        const int at = t + i * TPR;
+        place[i] = at < 16 ? begin + at : whole_to + (at - 16);
+        has_single[i] = at < 32 && place[i] < (at < 16 ? whole_from : end);
+        single_bits[i] = 0u;
+        if (has_single[i]) {
+            if constexpr (sizeof(T) == 2) single_bits[i] = __ldg(reinterpret_cast<const unsigned short*>(x) + place[i]);
+            else single_bits[i] = __ldg(reinterpret_cast<const uint32_t*>(x) + place[i]);
+        }
     }
     // A warp holds 32 NV groups in a row: its loads and stores differ by constants.
     const size_t first = g0 + t / 32 * (32 * NV) + t % 32;
     Group<T> held[NV];
-    uint32_t top = single_bits & (sizeof(T) == 2 ? 0x7FFFu : 0x7FFFFFFFu);
     #pragma unroll
     for (int j = 0; j < NV; ++j)
         if (first + j * 32 < g1) held[j].load(x, first + j * 32);
+    #pragma unroll
+    for (int i = 0; i < SINGLES; ++i) top = max(top, single_bits[i] & (sizeof(T) == 2 ? 0x7FFFu : 0x7FFFFFFFu));
     for (size_t group = g0 + t + NV * tpr; !WHOLE && group < g1; group += tpr) {
         Group<T> v;
         v.load(x, group);
@@ -181,7 +190,9 @@ int8_quantise_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float*
             reinterpret_cast<uint4*>(codes)[group] = c;
         }
     };
-    if (has_single) codes[single] = finite ? int8_t(code_of<T>(Bits<T>::widen(single_bits), s)) : int8_t(0);
+    #pragma unroll
+    for (int i = 0; i < SINGLES; ++i)
+        if (has_single[i]) codes[place[i]] = finite ? int8_t(code_of<T>(Bits<T>::widen(single_bits[i]), s)) : int8_t(0);
     #pragma unroll
     for (int j = 0; j < NV; ++j)
         if (first + j * 32 < g1) emit(held[j], first + j * 32);
@@ -253,7 +264,9 @@ void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, 
     constexpr bool SHORT = sizeof(T) == 2;
     constexpr int MOST = SHORT ? 4 : 2;
     if (K % 16 || groups > (SHORT ? 2048 : 1024)) {
-        if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
+        if (groups <= 8) go(int8_quantise_kernel<T, 8, 1, ROUTED, false>, 256, 32);
+        else if (groups <= 16) go(int8_quantise_kernel<T, 16, 1, ROUTED, false>, 256, 16);
+        else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
         else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, block(2, 256));
         else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, block(MOST, 512));
     } else if (groups <= 4) go(int8_quantise_kernel<T, 4, 1, ROUTED, true>, 256, 64);

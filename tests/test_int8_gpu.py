@@ -53,7 +53,8 @@ def check_quantised(g, x):
 @pytest.mark.parametrize("rows,k", ((1, 1), (3, 7), (9, 16), (5, 17), (33, 63), (17, 512), (10, 513), (4, 2048), (3, 2051),
                                     (3, 4096), (2, 8192), (2, 8191), (3, 16384), (2, 20000), (2, 32768), (2, 40001),
                                     (11, 1040), (3, 1552), (3, 2064), (3, 4112), (2, 4104), (2, 8784), (2, 8200), (2, 12304), (2, 14336),
-                                    (2, 16400), (2, 24592), (1, 16), (65, 48), (70, 64), (33, 80), (100, 128), (17, 144), (31, 256), (9, 272)))
+                                    (2, 16400), (2, 24592), (1, 16), (65, 48), (70, 64), (33, 80), (100, 128), (17, 144), (31, 256), (9, 272), (300, 1), (70, 15),
+                                    (65, 31), (33, 100), (37, 127), (33, 143), (35, 145), (50, 250), (17, 271), (18, 273)))
 def test_quantise(g, rows, k, dtype):
     check_quantised(g, normal((rows, k), dtype, rows * 7 + k))
 
