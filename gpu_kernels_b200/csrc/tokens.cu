@@ -281,42 +281,53 @@ tokens_gather_kernel(const T* __restrict__ x, T* __restrict__ rows, const int* _
 }
 
 // y[t] = sum over the live routes j of token t, in their order, of weights[t, j] * rows[position[t, j]] (weights null: of
-// the rows as they are, which is the gradient of the gather): FP32 sums, rounded once. GROUP rows are in flight at a time;
-// as few as topk needs, since registers are what bounds the loads in flight (4096 tokens of 4096 bf16 values, topk 6: with
-// room for eight 44 us, for six 37 us, 6.3 TB/s).
-template <typename T, int GROUP>
+// the rows as they are, which is the gradient of the gather): FP32 sums, rounded once. GROUP rows are in flight at a time,
+// PACKS packs of each: about eight loads, since fewer leave HBM waiting (rows of 4096 bf16 values: topk 1 takes 1.26 times
+// what its bytes take, with one pack in flight 1.73; topk 2 1.11 and 1.24) and registers bound the rest (topk 8 in two
+// rounds of four rows and two packs 1.09, with eight rows at once 1.31; topk 6 with six 1.14).
+template <typename T, int GROUP, int PACKS>
 __global__ void __launch_bounds__(ROW_THREADS)
 tokens_combine_kernel(const T* __restrict__ rows, const float* __restrict__ weights, const int* __restrict__ position,
                       const int* __restrict__ live, int tokens, int topk, int hidden, int segments, T* __restrict__ y) {
     ptx::chain_point();
     constexpr int N = 16 / int(sizeof(T));
-    const int token = blockIdx.x / segments;
-    const int p = (blockIdx.x - token * segments) * ROW_THREADS + threadIdx.x;
-    if (p >= hidden / N) return;
+    const int token = blockIdx.x / segments, packs = hidden / N;
+    const int p = (blockIdx.x - token * segments) * (ROW_THREADS * PACKS) + threadIdx.x;
+    if (p >= packs) return;
     const int end_live = min(__ldg(live), tokens * topk);
-    float sum[N];
+    float sum[PACKS][N];
     #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    for (int u = 0; u < PACKS; ++u)
+        #pragma unroll
+        for (int i = 0; i < N; ++i) sum[u][i] = 0.0f;
     for (int j0 = 0; j0 < topk; j0 += GROUP) {
-        Pack<T, N> v[GROUP];
+        Pack<T, N> v[GROUP][PACKS];
         bool there[GROUP];
         #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
             const int from = j0 + j < topk ? __ldg(position + size_t(token) * topk + j0 + j) : -1;
             there[j] = from >= 0 && from < end_live;
-            if (there[j]) v[j].load(rows + size_t(from) * hidden + size_t(p) * N);
+            #pragma unroll
+            for (int u = 0; u < PACKS; ++u)
+                if (there[j] && p + u * ROW_THREADS < packs) v[j][u].load(rows + size_t(from) * hidden + size_t(p + u * ROW_THREADS) * N);
         }
         #pragma unroll
         for (int j = 0; j < GROUP; ++j) {
             if (!there[j]) continue;
             const float w = weights ? __ldg(weights + size_t(token) * topk + j0 + j) : 1.0f;
             #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] = __fmaf_rn(w, v[j][i], sum[i]);
+            for (int u = 0; u < PACKS; ++u)
+                #pragma unroll
+                for (int i = 0; i < N; ++i) sum[u][i] = __fmaf_rn(w, v[j][u][i], sum[u][i]);
         }
     }
-    Pack<T, N> out;
-    out.set(sum);
-    out.store(y + size_t(token) * hidden + size_t(p) * N);
+    #pragma unroll
+    for (int u = 0; u < PACKS; ++u) {
+        if (p + u * ROW_THREADS >= packs) break;
+        Pack<T, N> out;
+        out.set(sum[u]);
+        out.store(y + size_t(token) * hidden + size_t(p + u * ROW_THREADS) * N);
+    }
 }
 
 // The same for rows of narrower packs (an odd number of values, say): eight packs of one row in flight per thread instead
@@ -601,14 +612,21 @@ void tokens_combine(const void* rows, int dtype, const float* weights, const int
     by_type(dtype, hidden, {rows, y}, [&](auto value, auto n) {
         using T = decltype(value);
         constexpr int N = decltype(n)::value;
-        int segments;
-        const unsigned grid = blocks(tokens, hidden / N, sizeof(T) * N == 16 ? ROW_THREADS : ROW_THREADS * NARROW, segments);
-        auto go = [&](auto kernel) {
+        auto go = [&](auto kernel, int packs) {                  // of a row, to a thread
+            int segments;
+            const unsigned grid = blocks(tokens, hidden / N, ROW_THREADS * packs, segments);
             launch_chained(kernel, dim3(grid), dim3(ROW_THREADS), 0, stream, static_cast<const T*>(rows), weights, position, live,
                            tokens, topk, hidden, segments, static_cast<T*>(y));
         };
-        if constexpr (sizeof(T) * N == 16) by_group(topk, [&](auto group) { go(tokens_combine_kernel<T, decltype(group)::value>); });
-        else go(tokens_combine_narrow_kernel<T, N>);
+        if constexpr (sizeof(T) * N == 16)
+            by_group(topk, [&](auto group) {
+                constexpr int GROUP = decltype(group)::value <= 6 ? decltype(group)::value : 4;
+                if constexpr (GROUP <= 4) {
+                    if (hidden / N > ROW_THREADS) return go(tokens_combine_kernel<T, GROUP, 2>, 2);
+                }
+                go(tokens_combine_kernel<T, GROUP, 1>, 1);
+            });
+        else go(tokens_combine_narrow_kernel<T, N>, NARROW);
     });
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
