@@ -270,8 +270,8 @@ def test_grouped_offsets_that_make_no_sense_stay_in_bounds(g):
 
 
 def test_matrices_beyond_31_bits(g):
-    # 70001 x 30728 values: the last rows lie behind element 2^31
-    rows, k, tail = 70001, 30728, slice(69990, None)
+    # 70001 x 30808 values: the last rows lie behind element 2^31
+    rows, k, tail = 70001, 30808, slice(69990, None)
     x = torch.empty((rows, k), dtype=BF16, device="cuda").normal_(generator=generator(1))
     codes, scales = g.quantize_int8(x)
     want, want_scales = codes_of(x[tail])

@@ -189,8 +189,8 @@ def test_gather_quantised(g, tokens, topk, experts, k, dtype):
 
 
 def test_rows_beyond_31_bits(g):
-    # 9000 tokens of eight routes, 30728 values a row: the last rows lie behind element 2^31
-    tokens, topk, experts, hidden = 9000, 8, 16, 30728
+    # 9000 tokens of eight routes, 30808 values a row: the last rows lie behind element 2^31
+    tokens, topk, experts, hidden = 9000, 8, 16, 30808
     routes = g.sort_routes(choices(tokens, topk, experts, 1), experts)
     x = torch.empty((tokens, hidden), dtype=BF16, device="cuda").normal_(generator=generator(2)).requires_grad_()
     rows = g.gather_tokens(x, routes)
