@@ -107,7 +107,10 @@ class _GatherTokens(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_rows):
-        return _combine(d_rows, _places(*ctx.saved_tensors), None), None, None, None
+        # What hooks (save_on_cpu, checkpointing) give back belongs to this call alone: held by name until the launch, which
+        # is given addresses.
+        position, offsets = ctx.saved_tensors
+        return _combine(d_rows, _places(position, offsets), None), None, None, None
 
 
 class _CombineTokens(torch.autograd.Function):
@@ -119,11 +122,11 @@ class _CombineTokens(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_y):
-        position, offsets, weights, rows = ctx.saved_tensors
+        position, offsets, weights, rows = ctx.saved_tensors                # (held until the launch, as above)
         places = _places(position, offsets)
         if weights is None:
             return _gather(d_y, places), None, None, None, None
-        position, live, tokens, topk = places
+        at_position, live, tokens, topk = places
         d_y = d_y.contiguous()
         hidden = d_y.shape[1]
         d_rows = d_weights = None
@@ -133,7 +136,7 @@ class _CombineTokens(torch.autograd.Function):
             d_weights = matrix(tokens, topk, torch.float32, d_y.device)
             rows = rows.contiguous()
         _lib.run(d_y.device, _lib.load().gpu_kernels_tokens_combine_backward, d_y.data_ptr(), _DTYPES[d_y.dtype],
-                 None if rows is None else rows.data_ptr(), weights.data_ptr(), position, live, tokens, topk, hidden,
+                 None if rows is None else rows.data_ptr(), weights.data_ptr(), at_position, live, tokens, topk, hidden,
                  None if d_rows is None else d_rows.data_ptr(), None if d_weights is None else d_weights.data_ptr())
         return d_rows, d_weights, None, None, None
 

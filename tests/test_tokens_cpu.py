@@ -1,0 +1,58 @@
+"""What the routing operators hand to their kernels, with the launches replaced: no GPU is needed."""
+import weakref
+
+import pytest
+import torch
+
+
+class Launches:
+    """Stands for `_lib.run`: checks, at each launch, that no address it is given lies in memory nobody holds any more.
+    `copy` makes the tensors that are looked after, in memory that lives as long as their storage."""
+
+    def __init__(self):
+        self.memory, self.calls = [], 0
+
+    def copy(self, t):
+        array = t.detach().numpy().copy()
+        self.memory.append((array.ctypes.data, array.nbytes, weakref.ref(array)))
+        return torch.from_numpy(array)
+
+    def __call__(self, device, fn, *args):
+        self.calls += 1
+        lost = [a for a in args for at, size, ref in self.memory if ref() is None and isinstance(a, int) and at <= a < at + size]
+        assert not lost, "a launch is given memory that nobody holds"
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    from gpu_kernels_b200 import _lib, tokens
+    stub = Launches()
+    monkeypatch.setattr(_lib, "run", stub)
+    monkeypatch.setattr(tokens, "_require_cuda", lambda t, name: None)
+    return stub
+
+
+def order(tokens, topk):
+    """The order of a batch that one expert takes."""
+    import gpu_kernels_b200 as g
+    routes = torch.arange(tokens * topk, dtype=torch.int32)
+    return g.Routes(torch.tensor([0, tokens * topk], dtype=torch.int32), routes.view(tokens, topk).clone(), routes)
+
+
+@pytest.mark.parametrize("what,weighted", (("gather", None), ("combine", None), ("combine", "rows"), ("combine", "weights"), ("combine", "both")))
+def test_backward_holds_what_its_launch_reads(launches, what, weighted):
+    # Saved tensors that hooks give back (as save_on_cpu and checkpointing do) belong to the backward pass alone.
+    import gpu_kernels_b200 as g
+    tokens, topk, hidden = 6, 3, 8
+    routes = order(tokens, topk)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, launches.copy):
+        if what == "gather":
+            leaf = torch.ones((tokens, hidden), requires_grad=True)
+            out = g.gather_tokens(leaf, routes)
+        else:
+            leaf = torch.ones((tokens * topk, hidden), requires_grad=weighted != "weights")
+            weights = None if weighted is None else torch.ones((tokens, topk), requires_grad=weighted != "rows")
+            out = g.combine_tokens(leaf, routes, weights)
+    before = launches.calls
+    out.backward(torch.ones_like(out))
+    assert launches.calls == before + 1 and len(launches.memory) >= 2
