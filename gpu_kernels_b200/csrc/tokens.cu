@@ -27,6 +27,7 @@ namespace {
 // the same blocks, adds up the counts of the blocks before its own.
 constexpr int SORT_MAX_EXPERTS = 1024;
 constexpr int SMALL = 256, BLOCK = 1024, SORT_WARPS = BLOCK / 32;
+constexpr size_t SORT_STATIC = SORT_WARPS * sizeof(int);        // tokens_sort_kernel's static shared memory, which counts as well
 
 template <typename Id>
 __device__ __forceinline__ int key_of(const Id* ids, long long i, int experts) {
@@ -96,7 +97,7 @@ tokens_sort_kernel(const Id* __restrict__ ids, int routes, int experts, int part
     extern __shared__ int counters[];                           // [SORT_WARPS][keys], then for each key, [keys] each:
     int* first = counters + SORT_WARPS * keys;                  // its routes in the blocks before, later its first row in this block
     int* others = first + keys;                                 // its routes in the other blocks
-    __shared__ int warp_sum[SORT_WARPS];
+    __shared__ int warp_sum[SORT_STATIC / sizeof(int)];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int i = threadIdx.x; i < (SORT_WARPS + 2) * keys; i += BLOCK) counters[i] = 0;
     __syncthreads();
@@ -564,7 +565,7 @@ void launch_sort(const Id* ids, int routes, int experts, int* offsets, int* posi
         g_launches.fetch_add(1, std::memory_order_relaxed);
     }
     const size_t smem = (SORT_WARPS + 2) * keys * sizeof(int);
-    if (smem > 48 * 1024) cuda_check(cudaFuncSetAttribute(tokens_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    if (smem + SORT_STATIC > 48 * 1024) cuda_check(cudaFuncSetAttribute(tokens_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
     launch_chained(tokens_sort_kernel<Id>, dim3(unsigned(blocks)), dim3(BLOCK), smem, stream, ids, routes, experts, part,
                    blocks > 1 ? counts : nullptr, offsets, position, source);
 }
