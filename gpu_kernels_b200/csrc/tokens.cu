@@ -550,6 +550,20 @@ void by_group(int topk, F&& body) {
     return body(std::integral_constant<int, 8>{});
 }
 
+size_t sort_memory(int experts) { return size_t(SORT_WARPS + 2) * (size_t(experts) + 1) * sizeof(int); }
+
+// The limit is the function's, all threads' alike: raised once per device, to what the most experts take, and never lowered.
+template <typename Id>
+void allow_sort_memory() {
+    static std::atomic<bool> allowed[64] = {};
+    int device = 0;
+    cuda_check(cudaGetDevice(&device));
+    const bool known = device >= 0 && device < 64;
+    if (known && allowed[device].load(std::memory_order_acquire)) return;
+    cuda_check(cudaFuncSetAttribute(tokens_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_memory(SORT_MAX_EXPERTS))));
+    if (known) allowed[device].store(true, std::memory_order_release);
+}
+
 template <typename Id>
 void launch_sort(const Id* ids, int routes, int experts, int* offsets, int* position, int* source, int* counts, cudaStream_t stream) {
     const size_t keys = size_t(experts) + 1;
@@ -564,8 +578,8 @@ void launch_sort(const Id* ids, int routes, int experts, int* offsets, int* posi
         launch_chained(tokens_count_kernel<Id>, dim3(unsigned(blocks)), dim3(BLOCK), keys * sizeof(int), stream, ids, routes, experts, part, counts);
         g_launches.fetch_add(1, std::memory_order_relaxed);
     }
-    const size_t smem = (SORT_WARPS + 2) * keys * sizeof(int);
-    if (smem + SORT_STATIC > 48 * 1024) cuda_check(cudaFuncSetAttribute(tokens_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    const size_t smem = sort_memory(experts);
+    if (smem + SORT_STATIC > 48 * 1024) allow_sort_memory<Id>();
     launch_chained(tokens_sort_kernel<Id>, dim3(unsigned(blocks)), dim3(BLOCK), smem, stream, ids, routes, experts, part,
                    blocks > 1 ? counts : nullptr, offsets, position, source);
 }
