@@ -2,10 +2,11 @@
 
 A router gives each token topk experts (`route`); a route is one of these choices. `sort_routes` orders the routes by
 expert, `gather_tokens` copies the tokens' rows into that order (`gather_tokens_int8` quantises them on the way),
-`combine_tokens` adds the experts' rows up again, weighted, token by token. Both copies have gradients; the order is
-stable and every sum is taken in the order of the routes, so results do not change from run to run. The work is done by
-csrc/tokens.cu and csrc/int8_quant.cu through the C ABI (include/operators_capi.h); CPU tensors are rejected. Everything
-is asynchronous on the current stream and may be captured into a CUDA graph; nothing reads the routes back to the host.
+`combine_tokens` adds the experts' rows up again, weighted, token by token. `gather_tokens` and `combine_tokens` have
+gradients, and refuse tensors with a forward-mode tangent; codes have neither. The order is stable and every sum is taken in
+the order of the routes, so results do not change from run to run. The work is done by csrc/tokens.cu and
+csrc/int8_quant.cu through the C ABI (include/operators_capi.h); CPU tensors are rejected. Everything is asynchronous on the
+current stream and may be captured into a CUDA graph; nothing reads the routes back to the host.
 (Capture a backward pass with leaves that no graph outside the capture still refers to: autograd accumulates into a leaf
 on the stream where it was first used.)
 """
@@ -14,6 +15,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -98,6 +100,11 @@ def _combine(rows, places, weights):
     return y
 
 
+def _tangent(*tensors) -> bool:
+    """Whether one of them has a tangent: the autograd functions then refuse the call."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _GatherTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, position, offsets, places):
@@ -147,7 +154,7 @@ def gather_tokens(x: torch.Tensor, routes: Routes) -> torch.Tensor:
     Gradient: x's is the sum of its live rows' gradients, in FP32 and the order of the routes, rounded once."""
     _values(x, "x")
     places = _check_routes(routes, x.shape[0], x.device)
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _tangent(x):
         return _GatherTokens.apply(x, routes.position, routes.offsets, places)
     return _gather(x, places)
 
@@ -180,6 +187,7 @@ def combine_tokens(rows: torch.Tensor, routes: Routes, weights: torch.Tensor | N
             raise ValueError("weights must be floating-point, [tokens, topk] and where the rows are")
         weights = weights.float().contiguous()
     places = _check_routes(routes, None, rows.device)
-    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+    if (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))
+            or forward_ad._current_level >= 0 and _tangent(rows, weights)):
         return _CombineTokens.apply(rows, weights, routes.position, routes.offsets, places)
     return _combine(rows, places, weights)

@@ -3,6 +3,7 @@ import weakref
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 
 class Launches:
@@ -56,3 +57,18 @@ def test_backward_holds_what_its_launch_reads(launches, what, weighted):
     before = launches.calls
     out.backward(torch.ones_like(out))
     assert launches.calls == before + 1 and len(launches.memory) >= 2
+
+
+def test_tangents_are_refused(launches):
+    import gpu_kernels_b200 as g
+    routes = order(6, 3)
+    x, rows, w = torch.ones((6, 8)), torch.ones((18, 8)), torch.ones((6, 3))
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: g.gather_tokens(dual(x), routes), lambda: g.combine_tokens(dual(rows), routes, w),
+                     lambda: g.combine_tokens(dual(rows), routes), lambda: g.combine_tokens(rows, routes, dual(w)),
+                     lambda: g.combine_tokens(rows, routes, dual(w.double()))):
+            with pytest.raises(NotImplementedError):
+                call()
+        # plain tensors inside a level are as they are outside
+        assert g.gather_tokens(x, routes).shape == (18, 8) and g.combine_tokens(rows, routes, w).shape == (6, 8)
