@@ -25,6 +25,12 @@ def matrix(rows: int, columns: int, dtype: torch.dtype, device) -> torch.Tensor:
     return torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=device)
 
 
+def check_width(columns: int) -> None:
+    """Rows are counted in 64 bits, their values in 31."""
+    if columns >> 31:
+        raise ValueError("rows of fewer than 2^31 values")
+
+
 def placed(t: torch.Tensor):
     """(t, its address), t contiguous and on a 16-byte boundary: as it is where it is that already, else a copy."""
     if not t.is_contiguous():
@@ -40,13 +46,14 @@ def _rows(values: torch.Tensor, name: str):
     _require_cuda(values, name)
     if values.dim() != 2:
         raise ValueError(f"{name} must be 2-D [rows, K]")
+    check_width(values.shape[1])
     if values.dtype not in _DTYPES:
         values = values.float()
     return placed(values.detach() if values.requires_grad else values)
 
 
 def quantize_int8(values: torch.Tensor):
-    """[rows, K] (bf16, fp16 or fp32; any K) -> (codes int8 [rows, K], scales fp32 [rows]).
+    """[rows, K] (bf16, fp16 or fp32; any K below 2^31) -> (codes int8 [rows, K], scales fp32 [rows]).
 
     scale = max|row| / 127; a code is the integer nearest to 127 * value / max|row|, ties to the even one. A zero row has
     scale 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN."""
@@ -62,6 +69,7 @@ def quantize_int8(values: torch.Tensor):
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """codes * scales[:, None] -> fp32 [rows, K]."""
     _operand(codes, "codes", 2)
+    check_width(codes.shape[1])
     codes, at_codes = placed(codes)
     rows, k = codes.shape
     device = codes.device
@@ -94,9 +102,11 @@ def _output(out, m, n, dtype, device) -> torch.Tensor:
     return out
 
 
-def _check_sizes(n: int, k: int, other_k: int) -> None:
+def _check_sizes(m: int, n: int, k: int, other_k: int) -> None:
     if k != other_k:
         raise ValueError("the operands disagree on K")
+    if m > 1 << 30 or n > 1 << 30:
+        raise ValueError("M and N up to 2^30")
     if n < 8 or n % 8 or k < 16 or k % 16 or k > MAX_K:
         raise ValueError(f"N must be a multiple of 8 and K a multiple of 16 up to {MAX_K}")
 
@@ -105,12 +115,12 @@ def int8_gemm(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales
               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """C [M, N] = (a [M, K] @ b [N, K].T) * a_scales[:, None] * b_scales, in out's type (or out_dtype).
 
-    Any M; N a multiple of 8, K a multiple of 16 up to 131056."""
+    M and N up to 2^30; N a multiple of 8, K a multiple of 16 up to 131056."""
     device = a.device
     _operand(a, "a", 2)
     _operand(b, "b", 2, device)
     (m, k), (n, k2) = a.shape, b.shape
-    _check_sizes(n, k, k2)
+    _check_sizes(m, n, k, k2)
     (a, at_a), (b, at_b) = placed(a), placed(b)
     a_scales, at_a_scales = _scales(a_scales, "a_scales", (m,), device)
     b_scales, at_b_scales = _scales(b_scales, "b_scales", (n,), device)
@@ -128,7 +138,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
     device, dtype = x.device, x.dtype
     _operand(weight, "weight", 2, device)
     (m, k), (n, k2) = x.shape, weight.shape
-    _check_sizes(n, k, k2)
+    _check_sizes(m, n, k, k2)
     weight, at_weight = placed(weight)
     weight_scales, at_scales = _scales(weight_scales, "weight_scales", (n,), device)
     out = _output(out, m, n, out_dtype or dtype, device)
@@ -150,7 +160,7 @@ def int8_grouped_gemm(rows: torch.Tensor, weights: torch.Tensor, row_scales: tor
     _operand(rows, "rows", 2)
     _operand(weights, "weights", 3, rows.device)
     (r, k), (experts, n, k2) = rows.shape, weights.shape
-    _check_sizes(n, k, k2)
+    _check_sizes(r, n, k, k2)
     if not 1 <= experts <= 1024:
         raise ValueError("1..1024 experts")
     if offsets.dtype != torch.int32 or offsets.shape != (experts + 1,) or offsets.device != rows.device:
@@ -168,6 +178,8 @@ def int8_grouped_gemm(rows: torch.Tensor, weights: torch.Tensor, row_scales: tor
 
 def int8_tiles(rows: int, n: int, k: int, experts: int = 0) -> dict:
     """What a product of these sizes runs on the current device (experts > 0: a grouped one)."""
+    if max(rows, n, k, experts) >> 31:
+        raise ValueError("sizes of fewer than 32 bits")
     info = (ctypes.c_int * 5)()
     _lib.check(_lib.load().gpu_kernels_int8_tiles(rows, n, k, experts, info))
     return dict(zip(("pair", "swap", "width", "split", "stages"), info))
