@@ -995,6 +995,11 @@ nvfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     if (threadIdx.x == 0 && !g.late_trigger) grid_launch_dependents();
     if (PROF && threadIdx.x == 0) g.prof[(size_t(CG == 2 ? blockIdx.x / 2u : blockIdx.x) * CG + rank) * PROF_WORDS + PROF_T_ENTER] = globaltimer_ns();
 
+    // A pair allocates Tensor Memory together: both CTAs have to be there before either begins, and stay until both have
+    // given it back. A CTA that is launched later than its partner (its SM still busy with the kernel in front, which
+    // programmatic launch allows) may otherwise never get out of its allocation. Arriving here and not just in front of the
+    // wait: linear 1000 x 8192 x 8192 36.5 -> 36.1 us.
+    if constexpr (CG == 2) { __syncwarp(); cluster_arrive(); }
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::STAGES; ++s) {
             mbar_init(smem_u32(&ctrl->full[s]), 1);
@@ -1005,10 +1010,7 @@ nvfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         ctrl->wait.abort = 0;
         mbar_init_fence();
     }
-    // A pair allocates Tensor Memory together: both CTAs have to be there before either begins, and stay until both have
-    // given it back. A CTA that is launched later than its partner (its SM still busy with the kernel in front, which
-    // programmatic launch allows) may otherwise never get out of its allocation.
-    if constexpr (CG == 2) { __syncwarp(); cluster_arrive(); cluster_wait(); }
+    if constexpr (CG == 2) { __syncwarp(); cluster_wait(); }
     if (warp == 4) {
         tmem_alloc<CG>(smem_u32(&ctrl->tmem_base), TMEM_COLS);
         if constexpr (CG == 1) tmem_relinquish<CG>();
