@@ -25,12 +25,6 @@ def matrix(rows: int, columns: int, dtype: torch.dtype, device) -> torch.Tensor:
     return torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=device)
 
 
-def check_width(columns: int) -> None:
-    """Rows are counted in 64 bits, their values in 31."""
-    if columns >> 31:
-        raise ValueError("rows of fewer than 2^31 values")
-
-
 def placed(t: torch.Tensor):
     """(t, its address), t contiguous and on a 16-byte boundary: as it is where it is that already, else a copy."""
     if not t.is_contiguous():
@@ -46,7 +40,6 @@ def _rows(values: torch.Tensor, name: str):
     _require_cuda(values, name)
     if values.dim() != 2:
         raise ValueError(f"{name} must be 2-D [rows, K]")
-    check_width(values.shape[1])
     if values.dtype not in _DTYPES:
         values = values.float()
     return placed(values.detach() if values.requires_grad else values)
@@ -59,6 +52,8 @@ def quantize_int8(values: torch.Tensor):
     scale 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that what is computed from it is NaN."""
     values, address = _rows(values, "values")
     rows, k = values.shape
+    if k >> 31:
+        raise ValueError("K must be below 2^31")
     device = values.device
     codes = matrix(rows, k, torch.int8, device)
     scales = torch.empty(rows, dtype=torch.float32, device=device)
@@ -69,9 +64,10 @@ def quantize_int8(values: torch.Tensor):
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """codes * scales[:, None] -> fp32 [rows, K]."""
     _operand(codes, "codes", 2)
-    check_width(codes.shape[1])
     codes, at_codes = placed(codes)
     rows, k = codes.shape
+    if k >> 31:
+        raise ValueError("K must be below 2^31")
     device = codes.device
     scales, at_scales = _scales(scales, "scales", (rows,), device)
     out = matrix(rows, k, torch.float32, device)

@@ -19,7 +19,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .int8 import check_width, matrix, placed
+from .int8 import matrix, placed
 from .nvfp4 import _DTYPES, _require_cuda
 
 
@@ -63,23 +63,24 @@ def _places(position: torch.Tensor, offsets: torch.Tensor) -> tuple[int, int, in
 def _check_routes(routes: Routes, tokens: int | None, device) -> tuple[int, int, int, int]:
     """The places of a checked order."""
     offsets, position = routes.offsets, routes.position
-    if position.dim() != 2 or position.shape[1] < 1 or (tokens is not None and position.shape[0] != tokens):
+    shape = position.shape
+    if len(shape) != 2 or shape[1] < 1 or (tokens is not None and shape[0] != tokens):
         raise ValueError("the routes are not those of this many tokens")
-    if position.numel() >> 31:
+    batch, topk = shape
+    if batch * topk >> 31:
         raise ValueError("fewer than 2^31 routes")
-    for name, t in (("offsets", offsets), ("position", position)):
+    for t in (offsets, position):
         if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"routes.{name} must be a contiguous int32 tensor on {device}")
+            raise ValueError(f"routes.{'offsets' if t is offsets else 'position'} must be a contiguous int32 tensor on {device}")
     if offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError("routes.offsets must hold one value per expert and one more")
-    return _places(position, offsets)
+    return position.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), batch, topk
 
 
 def _values(t: torch.Tensor, name: str) -> torch.Tensor:
     _require_cuda(t, name)
-    if t.dim() != 2 or t.dtype not in _DTYPES or t.shape[1] < 1:
-        raise ValueError(f"{name} must be a bf16, fp16 or fp32 tensor [rows, hidden]")
-    check_width(t.shape[1])
+    if t.dim() != 2 or t.dtype not in _DTYPES or not 1 <= t.shape[1] < 1 << 31:
+        raise ValueError(f"{name} must be a bf16, fp16 or fp32 tensor [rows, hidden], hidden below 2^31")
     return t
 
 
