@@ -82,6 +82,10 @@ struct Tile {
     int scale;                      // first channel in b_scale
 };
 
+// Grouped products are SWAP, and SWAP pairs are there for them only.
+template <int CG, bool SWAP>
+__device__ __forceinline__ bool grouped(const Args& g) { return SWAP && (CG == 2 || g.offsets); }
+
 // The sequence of tiles one CTA (pair, cluster) works through; every role walks the same one.
 template <int CG, bool SWAP>
 struct Walk {
@@ -91,23 +95,22 @@ struct Walk {
     int t, stride, tiles, expert;
     __device__ Walk(const Args& args, const int* ts, const int* rs, int unit, int units)
         : g(args), tile_start(ts), row_start(rs), t(unit), stride(units), expert(0) {
-        tiles = g.offsets ? ts[g.experts] : g.tiles_x * g.tiles_y;
+        tiles = grouped<CG, SWAP>(g) ? ts[g.experts] : g.tiles_x * g.tiles_y;
     }
     __device__ bool valid() const { return t < tiles; }
     __device__ void next() { t += stride; }
     __device__ Tile tile() {
         constexpr int X = 128 * CG;
         Tile r;
-        if (g.offsets) {
+        if (grouped<CG, SWAP>(g)) {
             while (tile_start[expert + 1] <= t) ++expert;
             const int row0 = row_start[2 * expert], row1 = row_start[2 * expert + 1], rows = row1 - row0, local = t - tile_start[expert];
-            int per = SWAP ? g.width : X;
-            const int count = (rows + per - 1) / per, channel_tile = local / count, token_tile = local - channel_tile * count;
-            if (SWAP) per = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);         // equal shares, no more than g.width
+            const int count = (rows + g.width - 1) / g.width, channel_tile = local / count, token_tile = local - channel_tile * count;
+            const int per = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);              // equal shares, no more than g.width
             r.token = row0 + token_tile * per;
             r.token_end = min(row1, r.token + per);
-            r.n = SWAP ? (r.token_end - r.token + 16 * CG - 1) / (16 * CG) * (16 * CG) : g.width;
-            r.channel = channel_tile * (SWAP ? X : g.width);
+            r.n = (r.token_end - r.token + 16 * CG - 1) / (16 * CG) * (16 * CG);
+            r.channel = channel_tile * X;
             r.scale = expert * g.N + r.channel;
         } else {
             // bands of `band` tiles along the M side, every other one backwards along the N side: the tiles in flight share
@@ -214,7 +217,7 @@ struct Roles {
             const Tile t = walk.tile();
             x = t.x + (CG == 2 ? rank * 128 : 0);
             y = t.y + (CG == 2 ? rank * (t.n / 2) : 0);
-            parts = SWAP && g.offsets ? (t.n / CG + g.y_box - 1) / g.y_box : 1;
+            parts = grouped<CG, SWAP>(g) ? (t.n / CG + g.y_box - 1) / g.y_box : 1;
             bytes = uint32_t(CG) * uint32_t(g.x_box + parts * g.y_box) * ROW_BYTES;
         }
         __device__ void next() {
@@ -560,8 +563,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     if (warp == 4) tmem_alloc<CG>(smem_u32(&ctrl->tmem_base), columns);
     if (warp == 5 && lane == 0) { prefetch_tensormap(&mapX); prefetch_tensormap(&mapY); }
     if (!g.early) chain_point();
-    if (g.offsets) {
-        const int per = SWAP ? g.width : 128 * CG, channel_tiles = (g.N + (SWAP ? 128 * CG : g.width) - 1) / (SWAP ? 128 * CG : g.width);
+    if (grouped<CG, SWAP>(g)) {
+        const int per = g.width, channel_tiles = (g.N + 128 * CG - 1) / (128 * CG);
         for (int e = threadIdx.x; e < g.experts; e += THREADS) row_start[2 * e + 1] = min(max(__ldcg(g.offsets + e + 1), 0), g.M);
         __syncthreads();
         if (warp == 0) {
@@ -623,7 +626,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         roles.send(tmem, smem_u32(room), column_scale, warp & 3, half, lane);
     } else {
         roles.drain(tmem, acc_stride, warp & 3, half, lane);
-        if (g.offsets && g.zero_rest) {
+        if (grouped<CG, SWAP>(g) && g.zero_rest) {
             const size_t row_packs = size_t(g.N) * (g.out == DTYPE_F32 ? 4 : 2) / 16;
             const int first = row_start[0], end = row_start[2 * g.experts - 1];
             uint4* packs = reinterpret_cast<uint4*>(g.c);
@@ -779,7 +782,7 @@ void run(const int8_t* a, const int8_t* b, const float* a_scales, const float* b
     // each. What a stage holds beyond them is whatever was there: any byte is a number, a row of the product depends on its
     // own row alone, and rows that do not exist are not stored.
     const int x_tile = t.pair ? 256 : 128, half = t.pair ? 2 : 1, few = round_up(M, 8);
-    const int x_box = t.swap || t.pair || experts ? 128 : std::min(128, few);
+    const int x_box = t.swap || t.pair ? 128 : std::min(128, few);
     const int y_box = !t.swap ? t.width / half : experts ? std::min(32, t.width) : std::min(t.width, few);
     Args g{};
     g.M = M;
@@ -807,8 +810,7 @@ void run(const int8_t* a, const int8_t* b, const float* a_scales, const float* b
     g.tiles_y = (y_rows + t.width - 1) / t.width;
     long long tiles = (long long)(g.tiles_x) * g.tiles_y;
     if (experts) {                                              // at most: every expert's last tile may be partial
-        const int per = t.swap ? t.width : x_tile;
-        tiles = ((long long)(M) / per + std::min(M, experts)) * (t.swap ? g.tiles_x : g.tiles_y);
+        tiles = ((long long)(M) / t.width + std::min(M, experts)) * g.tiles_x;
     }
     if (tiles > 0x3FFFFFFFll) throw std::invalid_argument("int8 gemm: too many tiles");
     const int fit = resident(t, device);

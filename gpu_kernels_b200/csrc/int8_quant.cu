@@ -253,6 +253,7 @@ void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, 
     auto go = [&](auto kernel, int threads, int per_block = 1) {
         launch_chained(kernel, dim3(unsigned((rows + per_block - 1) / per_block)), dim3(threads), 0, stream,
                        static_cast<const T*>(x), codes, scales, rows, K, position, live, topk);
+        g_launches.fetch_add(1, std::memory_order_relaxed);
     };
     const int groups = K / 16;
     // As many warps as hold the row, `most` threads at most.
@@ -264,28 +265,30 @@ void launch(const void* x, int8_t* codes, float* scales, long long rows, int K, 
     constexpr bool SHORT = sizeof(T) == 2;
     constexpr int MOST = SHORT ? 4 : 2;
     if (K % 16 || groups > (SHORT ? 2048 : 1024)) {
-        if (groups <= 8) go(int8_quantise_kernel<T, 8, 1, ROUTED, false>, 256, 32);
-        else if (groups <= 16) go(int8_quantise_kernel<T, 16, 1, ROUTED, false>, 256, 16);
-        else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
-        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, block(2, 256));
-        else go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, block(MOST, 512));
+        if constexpr (!ROUTED) {                                 // (routed rows are whole groups: here only the longest)
+            if (groups <= 8) return go(int8_quantise_kernel<T, 8, 1, ROUTED, false>, 256, 32);
+            if (groups <= 16) return go(int8_quantise_kernel<T, 16, 1, ROUTED, false>, 256, 16);
+            if (groups <= 64) return go(int8_quantise_kernel<T, 32, 2, ROUTED, false>, 256, 8);
+            if (groups <= 512) return go(int8_quantise_kernel<T, 256, 2, ROUTED, false>, block(2, 256));
+        }
+        go(int8_quantise_kernel<T, 512, MOST, ROUTED, false>, block(MOST, 512));
     } else if (groups <= 4) go(int8_quantise_kernel<T, 4, 1, ROUTED, true>, 256, 64);
     else if (groups <= 8) go(int8_quantise_kernel<T, 8, 1, ROUTED, true>, 256, 32);
     else if (groups <= 16) go(int8_quantise_kernel<T, 16, 1, ROUTED, true>, 256, 16);
     else if (groups <= 32) go(int8_quantise_kernel<T, 32, 1, ROUTED, true>, 256, 8);
     else if (groups <= 64) go(int8_quantise_kernel<T, 32, 2, ROUTED, true>, 256, 8);
-    else if (SHORT && groups <= 96) go(int8_quantise_kernel<T, 32, 3, ROUTED, true>, 256, 8);
-    else if (groups <= 32 * MOST) go(int8_quantise_kernel<T, 32, MOST, ROUTED, true>, 256, 8);
-    else if (groups <= 256 && !SHORT) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, block(1, 256));
-    else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, block(2, 256));
     else if constexpr (SHORT) {
-        if (groups <= 1024) go(int8_quantise_kernel<T, 256, 4, ROUTED, true>, block(4, 256));
+        if (groups <= 96) go(int8_quantise_kernel<T, 32, 3, ROUTED, true>, 256, 8);
+        else if (groups <= 128) go(int8_quantise_kernel<T, 32, 4, ROUTED, true>, 256, 8);
+        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, block(2, 256));
+        else if (groups <= 1024) go(int8_quantise_kernel<T, 256, 4, ROUTED, true>, block(4, 256));
         else go(int8_quantise_kernel<T, 512, 4, ROUTED, true>, block(4, 512));
     } else {
-        if (groups <= 768) go(int8_quantise_kernel<T, 512, 2, ROUTED, true>, block(2, 512));
+        if (groups <= 256) go(int8_quantise_kernel<T, 256, 1, ROUTED, true>, block(1, 256));
+        else if (groups <= 512) go(int8_quantise_kernel<T, 256, 2, ROUTED, true>, block(2, 256));
+        else if (groups <= 768) go(int8_quantise_kernel<T, 512, 2, ROUTED, true>, block(2, 512));
         else go(int8_quantise_kernel<T, 1024, 1, ROUTED, true>, block(1, 1024));
     }
-    g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
 template <bool ROUTED>

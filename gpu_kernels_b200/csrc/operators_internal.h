@@ -16,9 +16,9 @@ CUtensorMap byte_rows_map(const void* p, size_t rows, size_t row_bytes, int box_
 inline size_t dtype_bytes(int dtype) { return dtype == DTYPE_F32 ? 4 : 2; }
 
 // int8_quant.cu
-// x [rows, K] -> codes [rows, K] and scales [rows]; position != null: row t of x goes to the rows position[t * topk + j]
-// of codes and scales instead (see int8_gather).
+// x [rows, K] -> codes [rows, K] and scales [rows].
 void int8_quantise(const void* x, int dtype, int8_t* codes, float* scales, long long rows, int K, cudaStream_t stream);
+// The same, row t of x to the rows position[t * topk + j] of codes and scales; zeros from row *live on.
 void int8_gather(const void* x, int dtype, long long tokens, int topk, int K, const int* position, const int* live, int8_t* codes,
                  float* scales, cudaStream_t stream);
 void int8_dequantise(const int8_t* codes, const float* scales, float* out, long long rows, int K, cudaStream_t stream);
