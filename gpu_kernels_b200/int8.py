@@ -4,7 +4,9 @@ Beside the NVFP4 path, for weights that are kept in 8 bits. `quantize_int8` give
 scale per row, for activations (a row is a token) and weights (a row is an output channel) alike; `int8_gemm` multiplies
 two such matrices, `int8_linear` quantises the activations on the way, and `int8_grouped_gemm` multiplies rows sorted by
 expert (`gather_tokens_int8`) with the expert's own weights. The sums are exact 32-bit integers, the scaling is FP32.
-Nothing here has a gradient. The work is done by csrc/int8_quant.cu and csrc/int8_gemm.cu through the C ABI
+Nothing here has a gradient. Operands may have any strides and alignment, but one that is not contiguous or not on a 16-byte
+boundary is copied whole on every call (weights too, of all experts): keep weights contiguous, as torch allocates them. An
+`out` has to be contiguous and on a 16-byte boundary. The work is done by csrc/int8_quant.cu and csrc/int8_gemm.cu through the C ABI
 (include/operators_capi.h); CPU tensors are rejected. Everything is asynchronous on the current stream, may be captured
 into a CUDA graph and keeps nothing between calls; `check_int8` reports a product that gave up waiting inside the kernel.
 """

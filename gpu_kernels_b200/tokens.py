@@ -26,7 +26,10 @@ from .nvfp4 import _DTYPES, _require_cuda
 class Routes(NamedTuple):
     """The order of a batch's routes: offsets int32 [E + 1] (expert e's rows are [offsets[e], offsets[e + 1])), position
     int32 [T, topk] (each route's row) and source int32 [T * topk] (each row's route, token * topk + choice). Routes of no
-    expert have the rows from offsets[E] on."""
+    expert have the rows from offsets[E] on.
+
+    An order of a caller's own making has to be one too: every row the place of exactly one route. With others nothing is read
+    or written out of bounds, but a row that no position names is not written, and one that several name is written by each."""
     offsets: torch.Tensor
     position: torch.Tensor
     source: torch.Tensor

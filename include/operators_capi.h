@@ -55,8 +55,9 @@ int gpu_kernels_tokens_sort(const void* ids, int id_bytes, int routes, int exper
                             void* workspace, void* stream);
 size_t gpu_kernels_tokens_sort_workspace(int routes, int experts);
 /* rows [tokens * topk, hidden]: x [tokens, hidden] in that order; `live` points to the number of live rows
- * (offsets + experts); the rows behind are cleared. A position outside the rows is skipped. Pointers need the alignment of
- * their type only; 16-byte aligned rows are copied 16 bytes at a time. */
+ * (offsets + experts); the rows behind are cleared. Every row is the place of one route: a position outside the rows is
+ * skipped, a row that no position names is not written. Pointers need the alignment of their type only; 16-byte aligned rows
+ * are copied 16 bytes at a time. */
 int gpu_kernels_tokens_gather(const void* x, int dtype, int tokens, int topk, int hidden, const void* position, const void* live,
                               void* rows, void* stream);
 /* The same, quantised: codes [tokens * topk, K] and scales [tokens * topk]; K a multiple of 16. */
